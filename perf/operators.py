@@ -92,13 +92,14 @@ def draw(rng):
                     biases=rng.choice([0, 1, 40]), mask=rng.random() < 0.5)
     q = rng.choice([1, 1, 1, rng.randrange(2, 17), _log(rng, 17, 1531)])
     seqs = _log(rng, 1, 48) if q < 17 else _log(rng, 1, 6)
+    int8 = rng.random() < 0.5
     ctx = _log(rng, max(q, 16), 40037)
-    ctx = max(q, min(ctx, 120_000 * 32 // (kv * seqs)))  # cached tokens x k heads within the listed cases'
+    ctx = max(q, min(ctx, (4_500_000 if int8 else 2_250_000) // (kv * seqs)))  # the cache within the listed cases'
     while heads * q * seqs * ctx > 800_000_000 and seqs > 1:
         seqs -= 1
     ctx = max(q, min(ctx, 800_000_000 // (heads * q * seqs)))
     return dict(op=op, seqs=seqs, q=q, ctx=ctx, spread=rng.choice([0.0, 0.5, 0.9]), heads=heads, kv_heads=kv, hd=hd,
-                window=rng.choice([0, 0, 0, max(1, ctx // 3)]), int8=rng.random() < 0.5,
+                window=rng.choice([0, 0, 0, max(1, ctx // 3)]), int8=int8,
                 pad=rng.choice([0, 0, 1]) if seqs > 2 else 0, page=page)
 
 
