@@ -27,6 +27,9 @@ pub const RT_CTX_TRAIN: c_int = 0;
 pub const RT_CTX_FORWARD_ONLY: c_int = 1;
 pub const RT_DIST_DATA_PARALLEL: c_int = 0;
 pub const RT_DIST_TENSOR_PARALLEL: c_int = 1;
+pub const RT_ROPE_PLAIN: c_int = 0;
+pub const RT_ROPE_LINEAR: c_int = 1;
+pub const RT_ROPE_BANDS: c_int = 2;
 
 /// ModelConfig (crates/engine/src/model.rs:5-17).
 #[repr(C)]
@@ -130,6 +133,48 @@ pub struct rt_tokens {
     _p: [u8; 0],
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rt_rope {
+    pub cos: *const f32,
+    pub sin: *const f32,
+    pub n_pos: i32,
+    pub rot: i32,
+    pub half: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rt_kv_pages {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+    pub num_pages: i64,
+    pub page_size: i32,
+    pub kv_heads: i32,
+    pub hd: i32,
+    pub int8_rows: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rt_logit_rules {
+    pub hist: *const i32,
+    pub hist_start: *const i32,
+    pub n_prompt: *const i32,
+    pub n_hist: i64,
+    pub repetition: *const f32,
+    pub presence: *const f32,
+    pub frequency: *const f32,
+    pub bias_ids: *const i32,
+    pub bias_vals: *const f32,
+    pub bias_start: *const i32,
+    pub n_bias: i64,
+    pub mask: *const u32,
+    pub mask_ld: i64,
+}
+
 extern "C" {
     pub fn rt_ctx_create(cfg: *const rt_model_config, device: c_int, max_batch: c_int, flags: c_int, out: *mut *mut rt_ctx) -> c_int;
     pub fn rt_ctx_destroy(ctx: *mut rt_ctx) -> c_int;
@@ -194,6 +239,15 @@ extern "C" {
     pub fn rt_kernel_ce_bwd(logits: *const f32, row_lse: *const f32, tgt: *const u32, dl_bf16: *mut c_void, M: c_int, V: c_int, softcap: f32, scale: f32, stream: *mut c_void) -> c_int;
     pub fn rt_kernel_adam(param: *mut f32, grad: *const f32, m: *mut f32, v: *mut f32, param_bf16: *mut c_void, n: i64, t: u32, lr: f32, beta1: f32, beta2: f32, eps: f32, weight_decay: f32, grad_scale: f32, stream: *mut c_void) -> c_int;
     pub fn rt_kernel_l2norm(x: *const f32, n: i64, partials: *mut f32, out_norm: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn rt_rope_tables(cos_out: *mut f32, sin_out: *mut f32, n_pos: c_int, rot: c_int, theta: f64, scaling: c_int, factor: f64, low: f64, high: f64, trained_pos: c_int) -> c_int;
+    pub fn rt_kernel_qk_norm_rope_fwd(x: *const c_void, ldx: i64, out: *mut c_void, ldo: i64, pos: *const i32, rope: *const rt_rope, gamma_q: *const f32, gamma_k: *const f32, eps: f32, T: c_int, heads: c_int, kv_heads: c_int, v_heads: c_int, hd: c_int, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
+    pub fn rt_kernel_qk_norm_rope_bwd(dy: *const c_void, lddy: i64, x: *const c_void, ldx: i64, dx: *mut c_void, lddx: i64, pos: *const i32, rope: *const rt_rope, gamma_q: *const f32, gamma_k: *const f32, eps: f32, dgamma_q: *mut f32, dgamma_k: *mut f32, accumulate: c_int, partials: *mut f32, T: c_int, heads: c_int, kv_heads: c_int, v_heads: c_int, hd: c_int, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
+    pub fn rt_kernel_qk_norm_rope_bwd_partials(T: c_int, heads: c_int, kv_heads: c_int) -> c_int;
+    pub fn rt_kernel_kv_append(qkv: *const c_void, ldqkv: i64, q_out: *mut c_void, ldq: i64, pos: *const i32, slots: *const i32, rope: *const rt_rope, gamma_q: *const f32, gamma_k: *const f32, eps: f32, cache: *const rt_kv_pages, T: c_int, heads: c_int, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
+    pub fn rt_kernel_kv_gather(cache: *const rt_kv_pages, slots: *const i32, k_out: *mut c_void, v_out: *mut c_void, ldo: i64, T: c_int, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
+    pub fn rt_kernel_attention_paged(q: *const c_void, ldq: i64, out: *mut c_void, ldo: i64, lse2: *mut f32, cache: *const rt_kv_pages, page_table: *const i32, table_ld: i64, kv_lens: *const i32, q_start: *const i32, nseq: c_int, T: c_int, max_q: c_int, max_kv: c_int, heads: c_int, window: c_int, scale: f32, workspace: *mut c_void, workspace_bytes: i64, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
+    pub fn rt_kernel_attention_paged_workspace_bytes(hd: c_int) -> i64;
+    pub fn rt_kernel_logits_adjust(logits: *const f32, ldl: i64, out: *mut f32, ldo: i64, token: *mut i32, B: c_int, V: c_int, rules: *const rt_logit_rules, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
 }
 
 /// Status -> the reference's `.expect()` behaviour: panic with the library's message.

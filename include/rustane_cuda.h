@@ -403,6 +403,122 @@ RT_API int rt_kernel_adam(float* param, const float* grad, float* m, float* v, v
 /* Deterministic global L2 norm; partials: scratch of 1024 floats. */
 RT_API int rt_kernel_l2norm(const float* x, int64_t n, float* partials, float* out_norm, void* stream);
 
+/* ------------------------------------------------------- serving
+ * What a trained model needs to answer: rotary positions given per token (with
+ * per-head norms of q and k, also for training), a paged key/value cache,
+ * attention of new tokens over it, and the step from logits to a token.  The
+ * reference trains and evaluates only, so these have no counterpart in it.
+ * All take DEVICE pointers and a cudaStream_t and launch asynchronously on it;
+ * rows are 16-byte aligned with strides in elements, a multiple of 8 for bf16.
+ * dev_err (nullable) points to a zeroed device int: an index out of range
+ * (position, slot, page, length: 6; token id: 4) writes its code there and is
+ * skipped or replaced as stated, never followed; a bounded wait that ran out
+ * writes 1 to 3.  Sizes of zero are allowed and launch nothing. */
+
+/* Rotary tables [n_pos][rot / 2] fp32 on the device.  half 0: the pairs (2i,
+ * 2i + 1) rotate (the layout the model's own forward uses); 1: (i, i + rot / 2).
+ * rot % 16 == 0, rot <= hd; columns from rot on pass unrotated. */
+typedef struct rt_rope {
+  const float *cos, *sin;
+  int32_t n_pos, rot, half;
+} rt_rope;
+
+/* Paged cache: k, v [num_pages][kv_heads][page_size][hd] in bf16, or (int8_rows)
+ * int8 with k_scale, v_scale [num_pages][kv_heads][page_size] fp32 (value = code *
+ * scale).  page_size 16, 32, 64 or 128; hd 64 or 128.  Slot s of a token is row s %
+ * page_size of page s / page_size. */
+typedef struct rt_kv_pages {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int64_t num_pages;
+  int32_t page_size, kv_heads, hd, int8_rows;
+} rt_kv_pages;
+
+/* Host-side helper: fill HOST tables cos_out, sin_out [n_pos][rot / 2] with the angles
+ * p * theta^(-2i / rot), computed in double.  RT_ROPE_LINEAR divides every frequency by
+ * factor; RT_ROPE_BANDS divides those that turn less than `low` times over trained_pos
+ * positions, keeps those that turn more than `high` times, and blends linearly between
+ * (low, high, trained_pos are read by RT_ROPE_BANDS only). */
+#define RT_ROPE_PLAIN 0
+#define RT_ROPE_LINEAR 1
+#define RT_ROPE_BANDS 2
+RT_API int rt_rope_tables(float* cos_out, float* sin_out, int n_pos, int rot, double theta, int scaling, double factor,
+                          double low, double high, int trained_pos);
+
+/* x [T, ldx] bf16 holds heads q vectors, kv_heads k vectors and v_heads v vectors of hd
+ * (64 or 128) per token.  out = the q and k vectors, RMS-normed per head with gamma_q /
+ * gamma_k [hd] fp32 (both or neither) and rotated to pos[T]; v copied.  out may be x.  A
+ * position outside [0, n_pos) counts as 0 and sets dev_err. */
+RT_API int rt_kernel_qk_norm_rope_fwd(const void* x, int64_t ldx, void* out, int64_t ldo, const int32_t* pos,
+                                      const rt_rope* rope, const float* gamma_q, const float* gamma_k, float eps, int T,
+                                      int heads, int kv_heads, int v_heads, int hd, int* dev_err, void* stream);
+/* Its backward: dx from dy (the gradient of out) and the forward's x (null without
+ * gammas); dgamma_q, dgamma_k [hd] (accumulate ? += : =) summed over tokens and heads in a
+ * fixed order.  partials: scratch of rt_kernel_qk_norm_rope_bwd_partials(T, heads,
+ * kv_heads) * hd floats (null without gammas).  dx may be dy. */
+RT_API int rt_kernel_qk_norm_rope_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, void* dx, int64_t lddx,
+                                      const int32_t* pos, const rt_rope* rope, const float* gamma_q,
+                                      const float* gamma_k, float eps, float* dgamma_q, float* dgamma_k, int accumulate,
+                                      float* partials, int T, int heads, int kv_heads, int v_heads, int hd, int* dev_err,
+                                      void* stream);
+RT_API int rt_kernel_qk_norm_rope_bwd_partials(int T, int heads, int kv_heads);
+
+/* The same forward pass as it fills the cache: qkv [T, ldqkv] holds heads q and
+ * cache->kv_heads k and v vectors of cache->hd; q goes to q_out [T, ldq], k and v to
+ * slot slots[t] (-1: not cached; outside the cache: dev_err, not cached; distinct).  int8
+ * rows: scale = amax / 127, code = the nearest; a row with a NaN or infinity gets a NaN
+ * scale. */
+RT_API int rt_kernel_kv_append(const void* qkv, int64_t ldqkv, void* q_out, int64_t ldq, const int32_t* pos,
+                               const int32_t* slots, const rt_rope* rope, const float* gamma_q, const float* gamma_k,
+                               float eps, const rt_kv_pages* cache, int T, int heads, int* dev_err, void* stream);
+/* Read tokens back: k_out, v_out [T, ldo] bf16, kv_heads * hd columns; slot -1 gives zeros. */
+RT_API int rt_kernel_kv_gather(const rt_kv_pages* cache, const int32_t* slots, void* k_out, void* v_out, int64_t ldo,
+                               int T, int* dev_err, void* stream);
+
+/* Attention of new tokens over the cache, causal.  q, out [T, ld] bf16, heads * cache->hd
+ * columns; heads a multiple of cache->kv_heads.  Sequence s owns rows [q_start[s],
+ * q_start[s + 1]) (q_start[nseq + 1] ascending from 0 to T) and the first kv_lens[s] tokens
+ * of its pages page_table[s * table_ld + ..], the new tokens (already appended) last: row i
+ * of n sits at position kv_lens[s] - n + i and sees the keys up to its own, the last
+ * `window` of them if window > 0.  A row that sees none gives out = 0, lse2 = -inf.  lse2
+ * (nullable): [T, heads] log2 of the sum of exponentials.  max_q, max_kv: upper bounds of
+ * the new tokens and the length of any sequence; they choose the kernel and size the grid,
+ * and the work follows the device lengths.  A length outside [0, table_ld * page_size]
+ * counts as 0 and sets dev_err, a page outside the cache is read as page 0 and sets it.
+ * workspace: 16-byte aligned, rt_kernel_attention_paged_workspace_bytes(cache->hd) bytes, zeroed before
+ * its first use (and again after a bounded wait ran out); calls that share it run on one
+ * stream. */
+RT_API int rt_kernel_attention_paged(const void* q, int64_t ldq, void* out, int64_t ldo, float* lse2,
+                                     const rt_kv_pages* cache, const int32_t* page_table, int64_t table_ld,
+                                     const int32_t* kv_lens, const int32_t* q_start, int nseq, int T, int max_q,
+                                     int max_kv, int heads, int window, float scale, void* workspace,
+                                     int64_t workspace_bytes, int* dev_err, void* stream);
+RT_API int64_t rt_kernel_attention_paged_workspace_bytes(int hd);
+
+/* What changes a row of logits before a token is chosen; null: not applied.  hist: each
+ * row's tokens [hist_start[b], hist_start[b + 1]), the first n_prompt[b] of them the
+ * prompt's (null: none), the rest its answer's.  Bias entries [bias_start[b], bias_start[b +
+ * 1]) add up in list order where a token repeats.  mask: bit v % 32 of word [b * mask_ld + v
+ * / 32] set: token v allowed. */
+typedef struct rt_logit_rules {
+  const int32_t *hist, *hist_start, *n_prompt;
+  int64_t n_hist;
+  const float *repetition, *presence, *frequency; /* [B] each */
+  const int32_t* bias_ids;
+  const float* bias_vals;
+  const int32_t* bias_start;
+  int64_t n_bias;
+  const uint32_t* mask;
+  int64_t mask_ld;
+} rt_logit_rules;
+/* out [B, ldo] (may be logits) fp32: tokens that occur in hist divide a positive logit by
+ * repetition[b] and multiply another; those in the answer lose frequency * count + presence;
+ * then biases; then -inf where the mask forbids.  token (nullable): the first index of the
+ * row's largest value, -1 if nothing is above -inf (NaN is never chosen).  An id outside
+ * [0, V) is skipped and sets dev_err. */
+RT_API int rt_kernel_logits_adjust(const float* logits, int64_t ldl, float* out, int64_t ldo, int32_t* token, int B,
+                                   int V, const rt_logit_rules* rules, int* dev_err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

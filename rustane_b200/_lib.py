@@ -24,6 +24,8 @@ RT_ERR_ARG, RT_ERR_SHAPE, RT_ERR_CUDA, RT_ERR_OOM, RT_ERR_TOKEN, RT_ERR_DEVICE, 
 RT_CTX_TRAIN, RT_CTX_FORWARD_ONLY = 0, 1
 RT_DIST_DATA_PARALLEL, RT_DIST_TENSOR_PARALLEL = 0, 1
 
+RT_ROPE_PLAIN, RT_ROPE_LINEAR, RT_ROPE_BANDS = range(3)
+
 EPI_BF16, EPI_F32, EPI_F32_ACC, EPI_RESIDUAL, EPI_ROPE, EPI_SWIGLU, EPI_SWIGLU_BWD, EPI_BF16_ROWDOT = range(8)
 
 
@@ -46,6 +48,23 @@ class RtTimings(ctypes.Structure):
                                               "kernel_launches")]
 
 
+class RtRope(ctypes.Structure):
+    _fields_ = [("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p)] + [(n, ctypes.c_int32) for n in ("n_pos", "rot", "half")]
+
+
+class RtKvPages(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [("num_pages", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("page_size", "kv_heads", "hd", "int8_rows")]
+
+
+class RtLogitRules(ctypes.Structure):
+    _fields_ = [("hist", ctypes.c_void_p), ("hist_start", ctypes.c_void_p), ("n_prompt", ctypes.c_void_p),
+                ("n_hist", ctypes.c_int64), ("repetition", ctypes.c_void_p), ("presence", ctypes.c_void_p),
+                ("frequency", ctypes.c_void_p), ("bias_ids", ctypes.c_void_p), ("bias_vals", ctypes.c_void_p),
+                ("bias_start", ctypes.c_void_p), ("n_bias", ctypes.c_int64), ("mask", ctypes.c_void_p),
+                ("mask_ld", ctypes.c_int64)]
+
+
 c_int, c_int64, c_float, c_void_p, c_uint32 = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_uint32
 c_float_p = ctypes.POINTER(ctypes.c_float)
 c_uint32_p = ctypes.POINTER(ctypes.c_uint32)
@@ -53,6 +72,7 @@ c_uint8_p = ctypes.POINTER(ctypes.c_uint8)
 P_CFG = ctypes.POINTER(RtModelConfig)
 P_TC = ctypes.POINTER(RtTrainConfig)
 P_PTRS = ctypes.POINTER(RtModelPtrs)
+P_ROPE, P_KV = ctypes.POINTER(RtRope), ctypes.POINTER(RtKvPages)
 
 # name -> (restype, argtypes); must cover every function include/rustane_cuda.h declares
 SIGNATURES: dict[str, tuple] = {
@@ -132,6 +152,23 @@ SIGNATURES: dict[str, tuple] = {
     "rt_kernel_adam": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_uint32, c_float,
                                c_float, c_float, c_float, c_float, c_float, c_void_p]),
     "rt_kernel_l2norm": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "rt_rope_tables": (c_int, [c_float_p, c_float_p, c_int, c_int, ctypes.c_double, c_int, ctypes.c_double,
+                               ctypes.c_double, ctypes.c_double, c_int]),
+    "rt_kernel_qk_norm_rope_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, P_ROPE, c_void_p, c_void_p,
+                                           c_float, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "rt_kernel_qk_norm_rope_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, P_ROPE,
+                                           c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int, c_void_p, c_int,
+                                           c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "rt_kernel_qk_norm_rope_bwd_partials": (c_int, [c_int, c_int, c_int]),
+    "rt_kernel_kv_append": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, P_ROPE, c_void_p,
+                                    c_void_p, c_float, P_KV, c_int, c_int, c_void_p, c_void_p]),
+    "rt_kernel_kv_gather": (c_int, [P_KV, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p]),
+    "rt_kernel_attention_paged": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, P_KV, c_void_p, c_int64,
+                                          c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
+                                          c_void_p, c_int64, c_void_p, c_void_p]),
+    "rt_kernel_attention_paged_workspace_bytes": (c_int64, [c_int]),
+    "rt_kernel_logits_adjust": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int,
+                                        ctypes.POINTER(RtLogitRules), c_void_p, c_void_p]),
 }
 
 _lib = None

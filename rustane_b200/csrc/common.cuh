@@ -22,6 +22,7 @@ enum DeviceError : int {
   kDevTimeoutEpilogue = 3,
   kDevBadToken = 4,
   kDevBadShape = 5,
+  kDevBadIndex = 6,  // a position, slot, page or length out of range
 };
 
 // 4 s: far above any legitimate wait inside one kernel of this library.
