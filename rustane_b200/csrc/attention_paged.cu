@@ -6,131 +6,608 @@
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - max);  lse2 = log2 sum exp
 // A row that sees no key (L < n, or an unused batch slot) gives o = 0, lse2 = -inf.
 //
-// One warp per (token, head): the lanes hold the head dimension, 4 keys at a time.
-#include <math_constants.h>
-
-#include "common.cuh"
+// This file: up to 16 rows per key head (a decode step).  HBM-bound: K and V of every
+// visible token are read once, 2 hd bytes a token and head each (int8: hd + 4).  The rows
+// are one m16n8k16 tile, so the matrix instructions do 16 rows' work whatever the number
+// of rows; even so they need a few percent of their rate at the speed HBM delivers.
+//
+// Two CTAs an SM, 160 threads each: warp 4 streams 64-key blocks by TMA (one box per page
+// and 128 bytes of head, swizzled) into a ring of 96 KB; warps 0-3 take 16 keys of each
+// block for all rows, each with its own running maximum, sum and output, which meet in
+// the last block's ring slot when the item (or the CTA's part of it) ends.  P is rounded
+// to bf16 for the P V product (its sum is not): 2^-9 of each weight.  int8 rows become
+// bf16 exactly (|code| <= 127) on their way into the product; k's scale multiplies the
+// score, v's the weight, in fp32.
+#include "attention_paged.cuh"
 #include "kernels.h"
-#include "serving.h"
 
 namespace rt {
+namespace paged {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kBM = 16;   // rows per tile
+constexpr int kBK = 64;   // keys per block
+constexpr int kConsumers = 4;
+constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int kRingBytes = 96 * 1024;
 
-struct Params {
-  PagedAttnArgs a;
-  int64_t n_rows;  // cache rows: pages x kv_heads x page_size
-  int page_shift;
-  float scale_log2;
+template <int HD, bool I8>
+struct Cfg {
+  static constexpr int ROW = HD * (I8 ? 1 : 2);  // bytes of a key
+  static constexpr int TILE = kBK * ROW;
+  static constexpr int SCALES = I8 ? kBK * 4 : 0;
+  static constexpr int STAGE = 2 * TILE + 2 * SCALES;  // K, V, scales of k, of v
+  static constexpr int SLOT = (STAGE + 1023) / 1024 * 1024;
+  static constexpr int STAGES = kRingBytes / SLOT < 8 ? kRingBytes / SLOT : 8;
+  static constexpr int BOX = ROW < 128 ? ROW : 128;  // bytes of a row in one TMA box
+  static constexpr int BOXES = ROW / BOX;
+  // the four warps' outputs meet CHUNK columns at a time in the last block's slot
+  static constexpr int CHUNK = 2 * TILE / (kConsumers * kBM * 4) < HD ? 2 * TILE / (kConsumers * kBM * 4) : HD;
+  static constexpr int BAR = STAGES * SLOT;
+  static constexpr int ML = BAR + 256;                     // float [warp][row][2]
+  static constexpr int FIX = ML + kConsumers * kBM * 8;    // float [row][2] of recomputed rows
+  static constexpr int BYTES = FIX + kBM * 8 + 64 + 1024;  // + flags, alignment slack
 };
 
-// Keys [lo, hi) of one head for one row, one warp: running max m (log2 domain), sum l
-// and the lane's HD / 32 entries of the unnormalised output.
+// byte offset of 16-byte chunk ch of row r in a TMA-swizzled tile of kBK rows
+template <int ROW>
+__device__ __forceinline__ uint32_t tile_off(int r, int ch) {
+  if (ROW == 64) return r * 64 + ((ch ^ ((r >> 1) & 3)) << 4);
+  return (ch >> 3) * (kBK * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
 template <int HD, bool I8>
-__device__ void row_attend(const PagedAttnArgs& a, int page_shift, const int32_t* table, int kvh, const float (&q)[HD / 32],
-                           int lo, int hi, float scale_log2, float& m, float& l, float (&o)[HD / 32]) {
-  constexpr int E = HD / 32;
-  const int lane = threadIdx.x & 31;
-  for (int j = lo; j < hi; ++j) {
-    int64_t page = table[j >> page_shift];
-    if (page < 0 || page >= a.cache.num_pages) {
-      if (lane == 0) set_error(a.err, kDevBadIndex);
-      page = 0;
+__global__ void __launch_bounds__(kThreads, 2)
+    attn_paged_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                          const __grid_constant__ Params p, int min_blocks) {
+  using C = Cfg<HD, I8>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR);
+  uint64_t* empty = full + C::STAGES;
+  float* ml = reinterpret_cast<float*>(smem + C::ML);
+  float* fix = reinterpret_cast<float*>(smem + C::FIX);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::FIX + kBM * 8);
+  volatile int* is_last = abort_flag + 1;
+  volatile unsigned* nan_rows = reinterpret_cast<volatile unsigned*>(abort_flag + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PagedAttnArgs& a = p.a;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kConsumers);
     }
-    const int64_t at = (((page * a.cache.kv_heads + kvh) << page_shift) + (j & ((1 << page_shift) - 1)));
-    float k[E], v[E];
+    *abort_flag = 0;
+    *nan_rows = 0;
+    fence_mbar_init();
+  }
+  int64_t total;
+  int P;
+  Walk<kBM, kBK> w = start_walk<kBM, kBK, kThreads>(p, min_blocks, total, P);  // its barriers cover the init above
+
+  if (warp == kConsumers) {
+    // ------------------------------------------------------------------ producer
+    // lane i < boxes of a block loads `sub` keys: a page, or half of one of 128
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
+    const int ps = 1 << p.page_shift, sub = ps < kBK ? ps : kBK;
+    int g = 0;
+    bool ok = true;
+    for (; ok && w.more(); w.next()) {
+      if (w.empty()) continue;
+      const int32_t* table = a.table + w.s * a.table_ld;
+      const int cnt = w.count();
+      const int key00 = (w.blk0 + w.off) * kBK;
+      // this lane's page of a block (fetched one block ahead of its use), -1: no key of it is seen
+      auto my_page = [&](int b) {
+        const int key = key00 + b * kBK + lane * sub;
+        return b < cnt && lane * sub < kBK && key < w.hi && key + sub > w.lo ? page_of(p, table, key) : -1;
+      };
+      int page = my_page(0);
+      for (int b = 0; b < cnt; ++b, ++g) {
+        const int st = g % C::STAGES;
+        const int key0 = key00 + b * kBK;
+        const int ahead = my_page(b + 1);
+        bool go = mbar_wait(&empty[st], ((g / C::STAGES) & 1) ^ 1) && !*abort_flag;
+        if (!__all_sync(0xffffffffu, go)) {
+          ok = false;
+          break;
+        }
+        const int loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        uint8_t* slot = smem + st * C::SLOT;
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], loads * sub * (2 * C::ROW + (I8 ? 8 : 0)));
+        __syncwarp();
+        if (page >= 0) {
+          const int64_t row64 = ((static_cast<int64_t>(page) * a.cache.kv_heads + w.h) << p.page_shift) +
+                                ((key0 + lane * sub) & (ps - 1));
+          const int row = static_cast<int>(row64);
+          const uint32_t at = lane * sub * C::BOX;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int64_t i = at * HD + lane * E + e;
-      if (I8) {
-        k[e] = static_cast<float>(static_cast<const int8_t*>(a.cache.k)[i]);
-        v[e] = static_cast<float>(static_cast<const int8_t*>(a.cache.v)[i]);
-      } else {
-        k[e] = __bfloat162float(static_cast<const __nv_bfloat16*>(a.cache.k)[i]);
-        v[e] = __bfloat162float(static_cast<const __nv_bfloat16*>(a.cache.v)[i]);
+          for (int x = 0; x < C::BOXES; ++x) {
+            tma_load_2d(slot + x * (kBK * C::BOX) + at, &tm_k, &full[st], x * C::BOX, row);
+            tma_load_2d(slot + C::TILE + x * (kBK * C::BOX) + at, &tm_v, &full[st], x * C::BOX, row);
+          }
+          if (I8) {
+            uint8_t* sc = slot + 2 * C::TILE + lane * sub * 4;
+            bulk_load(sc, a.cache.k_scale + row64, sub * 4, &full[st]);
+            bulk_load(sc + C::SCALES, a.cache.v_scale + row64, sub * 4, &full[st]);
+          }
+        }
+        __syncwarp();
+        page = ahead;
       }
     }
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s += q[e] * k[e];
-#pragma unroll
-    for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    if (I8) s *= a.cache.k_scale[at];
-    s *= scale_log2;
-    const float m2 = fmaxf(m, s);
-    // a score of -inf under a running maximum of -inf adds nothing
-    const float f = m == m2 ? 1.f : exp2f(m - m2);
-    const float p = s == -CUDART_INF_F ? 0.f : exp2f(s - m2);
-    l = l * f + p;
-    const float pv = I8 ? p * a.cache.v_scale[at] : p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * f + pv * v[e];
-    m = m2;
+    if (!ok) {  // let copies still in flight land before the CTA exits
+      if (lane == 0) set_error(a.err, kDevTimeoutProducer);
+      *abort_flag = 1;
+      for (int x = g > C::STAGES ? g - C::STAGES : 0; x < g; ++x)
+        mbar_wait(&full[x % C::STAGES], (x / C::STAGES) & 1);
+    }
+    return;
   }
+
+  // -------------------------------------------------------------------- consumers
+  constexpr int KS = HD / 16;  // k-steps of Q K^T; groups of 16 output columns of P V
+  const int gr = lane >> 2, c = lane & 3;
+  const uint32_t ring = smem_u32(smem);
+  int g = 0;
+  bool ok = true;
+  for (; w.more(); w.next()) {
+    const int rows = w.rows(), cnt = w.count();
+    const int r0 = w.t * kBM;
+    auto q_ptr = [&](int r) {
+      const int i = (r0 + r) / p.G, hg = w.h * p.G + (r0 + r) % p.G;
+      return a.q + (w.q0 + i) * a.ldq + hg * HD;
+    };
+    auto write_row4 = [&](int r, int col, const float (&o)[4]) {
+      const int i = (r0 + r) / p.G, hg = w.h * p.G + (r0 + r) % p.G;
+      *reinterpret_cast<uint2*>(a.out + (w.q0 + i) * a.ldo + hg * HD + col) =
+          make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    };
+    auto write_lse = [&](int r, float v) {
+      const int i = (r0 + r) / p.G, hg = w.h * p.G + (r0 + r) % p.G;
+      if (a.lse2) a.lse2[static_cast<int64_t>(w.q0 + i) * a.heads + hg] = v;
+    };
+    // thread's share of the rows at the end: row er, columns 4 ec + 32 j
+    const int er = threadIdx.x >> 3, ec = threadIdx.x & 7;
+    if (w.empty()) {
+      if (er < rows) {
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int col = 4 * ec; col < HD; col += 32) write_row4(er, col, zero);
+        if (ec == 0) write_lse(er, -CUDART_INF_F);
+      }
+      continue;
+    }
+
+    // Q: rows gr and gr + 8.  An int8 key's 16 bytes of a k-step arrive 4 to a thread, so
+    // there the k index 2c, 2c + 1, 2c + 8, 2c + 9 stands for entries 4c .. 4c + 3.
+    uint32_t qa[KS][4];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int r = gr + 8 * hf;
+      const bool in = r < rows;
+      const __nv_bfloat16* q = q_ptr(in ? r : 0);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint32_t* x = reinterpret_cast<const uint32_t*>(q + ks * 16 + (I8 ? 4 * c : 2 * c));
+        qa[ks][hf] = in ? x[0] : 0u;
+        qa[ks][2 + hf] = in ? x[I8 ? 1 : 4] : 0u;
+      }
+    }
+    float o[2 * KS][4];
+#pragma unroll
+    for (int i = 0; i < 2 * KS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+    const int hi_r[2] = {w.row_hi(min(gr, rows - 1)), w.row_hi(min(gr + 8, rows - 1))};
+    const int lo_r[2] = {w.row_lo(min(gr, rows - 1)), w.row_lo(min(gr + 8, rows - 1))};
+    // keys that every row sees
+    const int lo_all = w.row_lo(rows - 1), hi_all = w.row_hi(0);
+
+    for (int b = 0; b < cnt; ++b, ++g) {
+      const int st = g % C::STAGES;
+      const int key0 = (w.blk0 + w.off + b) * kBK + warp * 16;  // the warp's keys
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[st], (g / C::STAGES) & 1) && !*abort_flag);
+      if (!ok) *abort_flag = 1;  // the loops run on without waiting: every warp meets the same barriers
+      const uint32_t slot = ring + st * C::SLOT;
+      if (ok && key0 < w.hi && key0 + 16 > w.lo) {
+        float s[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+        // ------------------------------------------------------------ S = Q K^T
+        if (!I8) {
+          const int key = warp * 16 + ((lane >> 4) << 3) + (lane & 7);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t kb[4];
+            ldsm4(slot + tile_off<C::ROW>(key, 2 * ks + ((lane >> 3) & 1)), kb);
+            mma16816(s[0], qa[ks], kb[0], kb[1]);
+            mma16816(s[1], qa[ks], kb[2], kb[3]);
+          }
+        } else {
+          const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+#pragma unroll
+          for (int ks = 0; ks < KS; ks += 2) {
+            uint32_t kb[4];
+            ldsm4(slot + tile_off<C::ROW>(key, ks + (lane >> 4)), kb);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              mma16816(s[x & 1], qa[ks + (x >> 1)], i8x2_bf16x2<0, 1>(kb[x]), i8x2_bf16x2<2, 3>(kb[x]));
+          }
+        }
+        // ------------------------------------------------- scale, mask, running maximum
+        float vs[2][2];
+        const bool masked = key0 < lo_all || key0 + 16 > hi_all;
+        if (I8) {
+          const float* sc = reinterpret_cast<const float*>(smem + st * C::SLOT + 2 * C::TILE) + warp * 16 + 2 * c;
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            const float2 ks2 = *reinterpret_cast<const float2*>(sc + 8 * nt);
+            const float2 vs2 = *reinterpret_cast<const float2*>(sc + kBK + 8 * nt);
+            vs[nt][0] = vs2.x;
+            vs[nt][1] = vs2.y;
+            s[nt][0] *= ks2.x;
+            s[nt][1] *= ks2.y;
+            s[nt][2] *= ks2.x;
+            s[nt][3] *= ks2.y;
+          }
+        }
+        uint32_t seen = 0xffu;  // bit 4 nt + e
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] *= p.scale_log2;
+        if (masked) {
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = key0 + 8 * nt + 2 * c + (e & 1);
+              if (key < lo_r[e >> 1] || key >= hi_r[e >> 1]) {
+                s[nt][e] = -CUDART_INF_F;
+                seen &= ~(1u << (4 * nt + e));
+              }
+            }
+        }
+        float mx[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          mx[hf] = fmaxf(fmaxf(s[0][2 * hf], s[0][2 * hf + 1]), fmaxf(s[1][2 * hf], s[1][2 * hf + 1]));
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
+        }
+        const bool grow0 = mx[0] > m[0] + kRescale, grow1 = mx[1] > m[1] + kRescale;
+        if (__any_sync(0xffffffffu, grow0 || grow1)) {
+          const float f0 = grow0 ? ex2_approx(m[0] - mx[0]) : 1.f, f1 = grow1 ? ex2_approx(m[1] - mx[1]) : 1.f;
+          if (grow0) m[0] = mx[0];
+          if (grow1) m[1] = mx[1];
+          l[0] *= f0;
+          l[1] *= f1;
+#pragma unroll
+          for (int i = 0; i < 2 * KS; ++i) {
+            o[i][0] *= f0;
+            o[i][1] *= f0;
+            o[i][2] *= f1;
+            o[i][3] *= f1;
+          }
+        }
+        // a maximum of -inf (nothing seen yet) is taken as 0: the weights come out 0
+        const float ms[2] = {m[0] == -CUDART_INF_F ? 0.f : m[0], m[1] == -CUDART_INF_F ? 0.f : m[1]};
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[nt][e] = ex2_approx(s[nt][e] - ms[e >> 1]);
+            l[e >> 1] += s[nt][e];
+            if (I8) {
+              s[nt][e] *= vs[nt][e & 1];
+              if (masked && !((seen >> (4 * nt + e)) & 1u)) s[nt][e] = 0.f;  // whatever the scale was
+            }
+          }
+        const uint32_t pa[4] = {pack_bf16x2(s[0][0], s[0][1]), pack_bf16x2(s[0][2], s[0][3]),
+                                pack_bf16x2(s[1][0], s[1][1]), pack_bf16x2(s[1][2], s[1][3])};
+        // ------------------------------------------------------------- O += P V
+        const uint32_t vt = slot + C::TILE;
+        const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+        if (!I8) {
+          // v of keys that no row sees counts as 0, whatever is there
+          uint32_t keep[2] = {~0u, ~0u};
+          const bool edge = key0 < w.lo || key0 + 16 > w.hi;
+          if (edge) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int k = key0 + 8 * x + 2 * c;
+              keep[x] = (k >= w.lo && k < w.hi ? 0xffffu : 0u) | (k + 1 >= w.lo && k + 1 < w.hi ? 0xffff0000u : 0u);
+            }
+          }
+#pragma unroll
+          for (int dg = 0; dg < KS; ++dg) {
+            uint32_t vb[4];
+            ldsm4t(vt + tile_off<C::ROW>(key, 2 * dg + (lane >> 4)), vb);
+            if (edge) {
+              vb[0] &= keep[0];
+              vb[1] &= keep[1];
+              vb[2] &= keep[0];
+              vb[3] &= keep[1];
+            }
+            mma16816(o[2 * dg], pa, vb[0], vb[1]);
+            mma16816(o[2 * dg + 1], pa, vb[2], vb[3]);
+          }
+        } else {
+          // 16 columns give two tiles: their even and their odd entries
+#pragma unroll
+          for (int dg = 0; dg < KS; dg += 2) {
+            uint32_t vb[4];
+            ldsm4t(vt + tile_off<C::ROW>(key, dg + (lane >> 4)), vb);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              mma16816(o[2 * (dg + x)], pa, i8x2_bf16x2<0, 2>(vb[2 * x]), i8x2_bf16x2<0, 2>(vb[2 * x + 1]));
+              mma16816(o[2 * (dg + x) + 1], pa, i8x2_bf16x2<1, 3>(vb[2 * x]), i8x2_bf16x2<1, 3>(vb[2 * x + 1]));
+            }
+          }
+        }
+      }
+      if (b + 1 < cnt) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+      }
+    }
+
+    // ------------------------------------------------------------ the warps' results meet
+    const int last = (g - 1) % C::STAGES;  // still held
+    float* buf = reinterpret_cast<float*>(smem + last * C::SLOT);
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+      if (c == 0) {
+        ml[(warp * kBM + gr + 8 * hf) * 2] = m[hf];
+        ml[(warp * kBM + gr + 8 * hf) * 2 + 1] = l[hf];
+      }
+    }
+    consumer_bar();
+    auto merged = [&](int r, float& mm, float& ll) {
+      mm = -CUDART_INF_F;
+#pragma unroll
+      for (int x = 0; x < kConsumers; ++x) mm = fmaxf(mm, ml[(x * kBM + r) * 2]);
+      const float base = mm == -CUDART_INF_F ? 0.f : mm;
+      ll = 0.f;
+#pragma unroll
+      for (int x = 0; x < kConsumers; ++x) ll += ml[(x * kBM + r) * 2 + 1] * ex2_approx(ml[(x * kBM + r) * 2] - base);
+    };
+    float f[2], dummy, em, el;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      merged(gr + 8 * hf, em, dummy);
+      f[hf] = ex2_approx(m[hf] - (em == -CUDART_INF_F ? 0.f : em));
+    }
+    merged(er, em, el);
+    const bool split = w.off > 0 || cnt < w.nb;
+    float* part = split ? partial_slot<kBM, HD>(p, blockIdx.x, w.off > 0 ? 0 : 1) : nullptr;
+    // columns of a row are swizzled in groups of 8 over the banks
+    auto buf_at = [&](int wp, int r, int col) { return (wp * kBM + r) * C::CHUNK + (col ^ ((r & (C::CHUNK / 8 - 1)) << 3)); };
+    float inv = el == 0.f ? 0.f : 1.f / el;
+#pragma unroll
+    for (int ch = 0; ch < HD / C::CHUNK; ++ch) {
+      if (ch) consumer_bar();
+#pragma unroll
+      for (int dg = ch * C::CHUNK / 16; dg < (ch + 1) * C::CHUNK / 16; ++dg)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int r = gr + 8 * hf, col = dg * 16 - ch * C::CHUNK;
+          const float x0 = o[2 * dg][2 * hf] * f[hf], x1 = o[2 * dg][2 * hf + 1] * f[hf],
+                      y0 = o[2 * dg + 1][2 * hf] * f[hf], y1 = o[2 * dg + 1][2 * hf + 1] * f[hf];
+          if (I8) {
+            *reinterpret_cast<float4*>(buf + buf_at(warp, r, col + 4 * c)) = make_float4(x0, y0, x1, y1);
+          } else {
+            *reinterpret_cast<float2*>(buf + buf_at(warp, r, col + 2 * c)) = make_float2(x0, x1);
+            *reinterpret_cast<float2*>(buf + buf_at(warp, r, col + 8 + 2 * c)) = make_float2(y0, y1);
+          }
+        }
+      consumer_bar();
+      float v[C::CHUNK / 32][4];
+      bool nan = false;
+#pragma unroll
+      for (int j = 0; j < C::CHUNK / 32; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[j][e] = 0.f;
+#pragma unroll
+        for (int x = 0; x < kConsumers; ++x) {
+          const float4 u = *reinterpret_cast<const float4*>(buf + buf_at(x, er, 4 * ec + 32 * j));
+          v[j][0] += u.x;
+          v[j][1] += u.y;
+          v[j][2] += u.z;
+          v[j][3] += u.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) nan = nan || isnan(v[j][e]);
+      }
+      if (!I8 && w.n > 1) {
+        // a row may have met a NaN or an infinity of a key that only a later row sees
+        if (nan && er < rows && ok) atomicOr(const_cast<unsigned*>(nan_rows), 1u << er);
+        consumer_bar();
+        const unsigned todo = *nan_rows;
+        if (todo) {
+          const int seg_lo = (w.blk0 + w.off) * kBK, seg_hi = seg_lo + cnt * kBK;
+          for (int r = warp; r < kBM; r += kConsumers) {
+            if (!((todo >> r) & 1u)) continue;
+            float rm, rl, ro[HD / 32];
+            row_attend<HD>(p, a.table + w.s * a.table_ld, w.h, q_ptr(r), max(w.row_lo(r), seg_lo),
+                           min(w.row_hi(r), seg_hi), rm, rl, ro);
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) buf[r * HD + lane * (HD / 32) + e] = ro[e];
+            if (lane == 0) {
+              fix[2 * r] = rm;
+              fix[2 * r + 1] = rl;
+            }
+          }
+          consumer_bar();
+          if ((todo >> er) & 1u) {
+            em = fix[2 * er];
+            el = fix[2 * er + 1];
+            inv = el == 0.f ? 0.f : 1.f / el;
+#pragma unroll
+            for (int j = 0; j < C::CHUNK / 32; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[j][e] = buf[er * HD + 4 * ec + 32 * j + e];
+          }
+          if (threadIdx.x == 0) *nan_rows = 0;
+          consumer_bar();
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < C::CHUNK / 32; ++j) {
+        const int col = ch * C::CHUNK + 4 * ec + 32 * j;
+        if (split) {
+          __stcg(reinterpret_cast<float4*>(part + er * HD + col), make_float4(v[j][0], v[j][1], v[j][2], v[j][3]));
+        } else if (er < rows && ok) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j][e] = el == 0.f ? 0.f : v[j][e] * inv;
+          write_row4(er, col, v[j]);
+        }
+      }
+    }
+    fence_proxy_async_smem();  // the slot was written by threads; TMA writes it next
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[last]);
+    if (ec == 0) {
+      if (split) {
+        __stcg(part + kBM * HD + er, em);
+        __stcg(part + kBM * HD + kBM + er, el);
+      } else if (er < rows && ok) {
+        write_lse(er, el == 0.f ? -CUDART_INF_F : em + log2f(el));
+      }
+    }
+    if (!split) continue;
+
+    // -------------------------------------------- the item's CTAs: the last one joins them
+    const int64_t first_block = w.g - w.off;
+    const int cta0 = block_owner(first_block, total, P), cta1 = block_owner(first_block + w.nb - 1, total, P);
+    int* counter = static_cast<int*>(a.workspace) + cta0;
+    __threadfence();
+    consumer_bar();
+    if (threadIdx.x == 0) *is_last = atomicAdd(counter, 1) == cta1 - cta0;
+    consumer_bar();
+    if (!*is_last) continue;
+    __threadfence();
+    auto slot_of = [&](int cta) { return partial_slot<kBM, HD>(p, cta, cta == cta0 ? 1 : 0); };
+    float jm = -CUDART_INF_F, jl = 0.f, v[HD / 32][4];
+    for (int x = cta0; x <= cta1; ++x) jm = fmaxf(jm, __ldcg(slot_of(x) + kBM * HD + er));
+    const float base = jm == -CUDART_INF_F ? 0.f : jm;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = 0.f;
+    for (int x = cta0; x <= cta1; ++x) {
+      const float* src = slot_of(x);
+      const float wt = ex2_approx(__ldcg(src + kBM * HD + er) - base);
+      jl += wt * __ldcg(src + kBM * HD + kBM + er);
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) {
+        const float4 u = __ldcg(reinterpret_cast<const float4*>(src + er * HD + 4 * ec + 32 * j));
+        v[j][0] += wt * u.x;
+        v[j][1] += wt * u.y;
+        v[j][2] += wt * u.z;
+        v[j][3] += wt * u.w;
+      }
+    }
+    if (er < rows && ok) {
+      const float jinv = jl == 0.f ? 0.f : 1.f / jl;
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[j][e] = jl == 0.f ? 0.f : v[j][e] * jinv;
+        write_row4(er, 4 * ec + 32 * j, v[j]);
+      }
+      if (ec == 0) write_lse(er, jl == 0.f ? -CUDART_INF_F : jm + log2f(jl));
+    }
+    if (threadIdx.x == 0) *counter = 0;
+    consumer_bar();  // is_last is read before it is written again
+  }
+  if (!ok && threadIdx.x == 0) set_error(a.err, kDevTimeoutEpilogue);
 }
 
 template <int HD, bool I8>
-__global__ void __launch_bounds__(256) attn_paged_row_kernel(const Params p) {
-  constexpr int E = HD / 32;
-  const PagedAttnArgs& a = p.a;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int tok = static_cast<int>(item / a.heads), h = static_cast<int>(item % a.heads);
-  if (tok >= a.T) return;
-  int s = 0;
-  while (s + 1 < a.nseq && a.q_start[s + 1] <= tok) ++s;
-  const int t0 = a.q_start[s], t1 = a.q_start[s + 1];
-  const int kvh = h / (a.heads / a.cache.kv_heads);
-  float q[E], o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = __bfloat162float(a.q[tok * a.ldq + h * HD + lane * E + e]);
-    o[e] = 0.f;
-  }
-  int len = a.kv_lens[s];
-  if (len < 0 || len > a.table_ld << p.page_shift) {
-    if (lane == 0) set_error(a.err, kDevBadIndex);
-    len = 0;
-  }
-  const int hi = len - (t1 - t0) + (tok - t0) + 1;
-  const int lo = a.window > 0 ? max(0, hi - a.window) : 0;
-  float m = -CUDART_INF_F, l = 0.f;
-  if (tok >= t0 && tok < t1)
-    row_attend<HD, I8>(a, p.page_shift, a.table + s * a.table_ld, kvh, q, lo, hi, p.scale_log2, m, l, o);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    a.out[tok * a.ldo + h * HD + lane * E + e] = __float2bfloat16(l == 0.f ? 0.f : o[e] * inv);
-  if (a.lse2 && lane == 0)
-    a.lse2[static_cast<int64_t>(tok) * a.heads + h] = l == 0.f ? -CUDART_INF_F : m + log2f(l);
+int launch(const Params& p, cudaStream_t s) {
+  using C = Cfg<HD, I8>;
+  CUtensorMap tk, tv;
+  const uint64_t rows = static_cast<uint64_t>(p.a.cache.num_pages) * p.a.cache.kv_heads * p.a.cache.page_size;
+  const uint32_t box = p.a.cache.page_size < kBK ? p.a.cache.page_size : kBK;
+  if (!make_tmap_rows(&tk, p.a.cache.k, C::ROW, rows, C::BOX, box) ||
+      !make_tmap_rows(&tv, p.a.cache.v, C::ROW, rows, C::BOX, box))
+    return -3;
+  const void* fn = reinterpret_cast<const void*>(attn_paged_few_kernel<HD, I8>);
+  const cudaError_t attr = smem_limit_once(fn, C::BYTES);
+  if (attr != cudaSuccess) return attr;
+  // no more CTAs than the bounds allow blocks (a sequence without keys costs one)
+  const int64_t tiles = (static_cast<int64_t>(p.a.max_q < 1 ? 1 : p.a.max_q) * p.G + kBM - 1) / kBM;
+  const int64_t keys = p.a.max_kv < 1 ? 1 : p.a.max_kv;
+  const int64_t most = p.a.nseq * static_cast<int64_t>(p.a.cache.kv_heads) * tiles * ((keys + kBK - 1) / kBK);
+  const int64_t ctas = attn_paged_few_ctas();
+  attn_paged_few_kernel<HD, I8><<<static_cast<unsigned>(most < ctas ? most : ctas), kThreads, C::BYTES, s>>>(tk, tv, p, 1);
+  return cudaGetLastError();
 }
 
 }  // namespace
+}  // namespace paged
 
-int64_t attn_paged_workspace_bytes(int) { return 4096; }
+int64_t attn_paged_few_ctas() {
+  const int c = 2 * num_sms();
+  return c < paged::kMaxCtas ? c : paged::kMaxCtas;
+}
+
+int attn_paged_few(const paged::Params& p, cudaStream_t s) {
+  if (p.a.cache.hd == 128) return p.a.cache.int8 ? paged::launch<128, true>(p, s) : paged::launch<128, false>(p, s);
+  return p.a.cache.int8 ? paged::launch<64, true>(p, s) : paged::launch<64, false>(p, s);
+}
+
+int64_t attn_paged_workspace_bytes(int hd) {
+  return paged::kCounterBytes + attn_paged_few_ctas() * 2 * paged::kBM * (hd + 2) * 4;
+}
 
 int attn_paged(const PagedAttnArgs& a, cudaStream_t s) {
   if (!kv_pages_ok(a.cache) || a.nseq < 0 || a.T < 0 || a.heads <= 0 || a.heads % a.cache.kv_heads) return -1;
   const int64_t cols = static_cast<int64_t>(a.heads) * a.cache.hd;
   if (a.ldq % 8 || a.ldo % 8 || a.ldq < cols || a.ldo < cols || a.table_ld < 0 || a.window < 0) return -1;
-  if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15) return -1;
+  if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.workspace)) & 15)
+    return -1;
   if (a.workspace_bytes < attn_paged_workspace_bytes(a.cache.hd)) return -1;
+  if (static_cast<int64_t>(a.T) * a.heads >= int64_t(1) << 31) return -1;  // rows are counted in 32 bits
   if (a.T == 0 || a.nseq == 0) return 0;
-  Params p;
+  paged::Params p;
   p.a = a;
-  p.n_rows = a.cache.num_pages * a.cache.kv_heads * a.cache.page_size;
+  p.G = a.heads / a.cache.kv_heads;
   p.page_shift = 31 - __builtin_clz(a.cache.page_size);
-  p.scale_log2 = a.scale * kLog2e;
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(a.T) * a.heads + 7) / 8);
-  if (a.cache.hd == 128) {
-    if (a.cache.int8) attn_paged_row_kernel<128, true><<<grid, 256, 0, s>>>(p);
-    else attn_paged_row_kernel<128, false><<<grid, 256, 0, s>>>(p);
-  } else {
-    if (a.cache.int8) attn_paged_row_kernel<64, true><<<grid, 256, 0, s>>>(p);
-    else attn_paged_row_kernel<64, false><<<grid, 256, 0, s>>>(p);
-  }
-  return cudaGetLastError();
+  const int64_t room = a.table_ld * a.cache.page_size;
+  p.max_len = static_cast<int>(room < (1 << 30) ? room : 1 << 30);
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  return attn_paged_few(p, s);
 }
 
 }  // namespace rt

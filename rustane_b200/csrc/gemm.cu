@@ -997,6 +997,18 @@ bool make_tmap_bf16(CUtensorMap* tm, const void* ptr, uint64_t inner, uint64_t o
   return encoder_ready() && make_tmap(tm, ptr, inner, outer, ld, box_inner, box_outer);
 }
 
+bool make_tmap_rows(CUtensorMap* tm, const void* ptr, uint64_t row_bytes, uint64_t rows, uint32_t box_bytes,
+                    uint32_t box_rows) {
+  if (!encoder_ready()) return false;
+  cuuint64_t dims[2] = {row_bytes, rows};
+  cuuint64_t strides[1] = {row_bytes};
+  cuuint32_t box[2] = {box_bytes, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int gemm_launch(const GemmArgs& g, cudaStream_t stream) {
   if (!encoder_ready()) return -2;
   if (g.M <= 0 || g.N <= 0 || g.K <= 0 || g.K % BK != 0 || g.N % 32 != 0) return -1;

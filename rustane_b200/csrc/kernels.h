@@ -68,6 +68,9 @@ int gemm_launch(const GemmArgs& g, cudaStream_t stream);
 // boxes of box_inner x box_outer; false if the driver entry point is missing.
 bool make_tmap_bf16(CUtensorMap* tm, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld,
                     uint32_t box_inner, uint32_t box_outer);
+// Contiguous rows of row_bytes, in boxes of box_bytes (64 or 128, swizzled by as much) x box_rows.
+bool make_tmap_rows(CUtensorMap* tm, const void* ptr, uint64_t row_bytes, uint64_t rows, uint32_t box_bytes,
+                    uint32_t box_rows);
 int num_sms();
 // Floats a GemmArgs::sumsq buffer needs (8 per SM).
 int gemm_sumsq_slots();

@@ -487,7 +487,7 @@ bool kv_pages_ok(const KvPages& c) {
   if (c.page_size < 16 || c.page_size > 128 || log2_exact(c.page_size) < 0) return false;
   // rows (page, head, token) are TMA coordinates and slots are int32
   if (c.num_pages > (int64_t(1) << 31) / (static_cast<int64_t>(c.kv_heads) * c.page_size) - 1) return false;
-  if (!aligned16(c.k) || !aligned16(c.v)) return false;
+  if (!aligned16(c.k) || !aligned16(c.v) || !aligned16(c.k_scale) || !aligned16(c.v_scale)) return false;
   return true;
 }
 
