@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   int64_t total;
   int P;
-  Walk<kBM, kBK> w = start_walk<kBM, kBK, kThreads>(p, min_blocks, total, P);  // its barriers cover the init above
+  Walk<kBK> w = start_walk<kBK, kThreads>(p, min_blocks, total, P);  // its barriers cover the init above
 
   if (warp == kConsumers) {
     // ------------------------------------------------------------------ producer
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int j = 0; j < C::CHUNK / 32; ++j) {
         const int col = ch * C::CHUNK + 4 * ec + 32 * j;
         if (split) {
-          __stcg(reinterpret_cast<float4*>(part + er * HD + col), make_float4(v[j][0], v[j][1], v[j][2], v[j][3]));
+          if (er < rows) __stcg(reinterpret_cast<float4*>(part + er * HD + col), make_float4(v[j][0], v[j][1], v[j][2], v[j][3]));
         } else if (er < rows && ok) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[j][e] = el == 0.f ? 0.f : v[j][e] * inv;
@@ -518,13 +518,14 @@ __global__ void __launch_bounds__(kThreads, 2)
     __threadfence();
     auto slot_of = [&](int cta) { return partial_slot<kBM, HD>(p, cta, cta == cta0 ? 1 : 0); };
     float jm = -CUDART_INF_F, jl = 0.f, v[HD / 32][4];
-    for (int x = cta0; x <= cta1; ++x) jm = fmaxf(jm, __ldcg(slot_of(x) + kBM * HD + er));
+    const int parts_end = er < rows ? cta1 : cta0 - 1;
+    for (int x = cta0; x <= parts_end; ++x) jm = fmaxf(jm, __ldcg(slot_of(x) + kBM * HD + er));
     const float base = jm == -CUDART_INF_F ? 0.f : jm;
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[j][e] = 0.f;
-    for (int x = cta0; x <= cta1; ++x) {
+    for (int x = cta0; x <= parts_end; ++x) {
       const float* src = slot_of(x);
       const float wt = ex2_approx(__ldcg(src + kBM * HD + er) - base);
       jl += wt * __ldcg(src + kBM * HD + kBM + er);
@@ -588,13 +589,15 @@ int attn_paged_few(const paged::Params& p, cudaStream_t s) {
 }
 
 int64_t attn_paged_workspace_bytes(int hd) {
-  return paged::kCounterBytes + attn_paged_few_ctas() * 2 * paged::kBM * (hd + 2) * 4;
+  const int64_t few = attn_paged_few_ctas() * paged::kBM, many = attn_paged_many_ctas() * 128;
+  return paged::kCounterBytes + (few > many ? few : many) * 2 * (hd + 2) * 4;
 }
 
 int attn_paged(const PagedAttnArgs& a, cudaStream_t s) {
   if (!kv_pages_ok(a.cache) || a.nseq < 0 || a.T < 0 || a.heads <= 0 || a.heads % a.cache.kv_heads) return -1;
   const int64_t cols = static_cast<int64_t>(a.heads) * a.cache.hd;
   if (a.ldq % 8 || a.ldo % 8 || a.ldq < cols || a.ldo < cols || a.table_ld < 0 || a.window < 0) return -1;
+  if (!(a.scale > 0.f)) return -1;
   if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.workspace)) & 15)
     return -1;
   if (a.workspace_bytes < attn_paged_workspace_bytes(a.cache.hd)) return -1;
@@ -607,7 +610,14 @@ int attn_paged(const PagedAttnArgs& a, cudaStream_t s) {
   const int64_t room = a.table_ld * a.cache.page_size;
   p.max_len = static_cast<int>(room < (1 << 30) ? room : 1 << 30);
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  return attn_paged_few(p, s);
+  // Up to 16 rows per key head and sequence fill one tile of the kernel above; more rows share
+  // each block's keys in tiles of up to 128 on the tcgen05 tensor cores.
+  if (static_cast<int64_t>(a.max_q) * p.G <= paged::kBM || p.G > 128) {
+    p.bm = paged::kBM;
+    return attn_paged_few(p, s);
+  }
+  p.bm = 128 / p.G * p.G;  // whole tokens, so that a tile of q is one TMA box
+  return attn_paged_many(p, s);
 }
 
 }  // namespace rt

@@ -3,7 +3,7 @@
 // join of an item that several CTAs worked on, and the one-row fallback.
 //
 // Rows.  Of sequence s and key head h, row r = i * G + g is new token i of query head h * G +
-// g (G = heads / kv_heads); a tile is BM consecutive rows, an item (s, h, tile).  Keys come
+// g (G = heads / kv_heads); a tile is bm consecutive rows, an item (s, h, tile).  Keys come
 // in blocks of BK; an item costs the blocks that any of its rows sees, one if none.
 //
 // Split.  All items' blocks, in order (s, h, tile, block), are cut into P equal ranges, one
@@ -29,6 +29,7 @@ constexpr float kRescale = 8.0f;  // keep a running maximum that is at most 2^8 
 struct Params {
   PagedAttnArgs a;
   int G;           // query heads per key head
+  int bm;          // rows per tile
   int page_shift;
   int max_len;     // tokens a row of the page table holds
   float scale_log2;
@@ -42,7 +43,7 @@ __device__ __forceinline__ float* partial_slot(const Params& p, int cta, int whi
 }
 
 // Walks one CTA's range of blocks, item by item.
-template <int BM, int BK>
+template <int BK>
 struct Walk {
   const Params* p;
   int s, h, t;            // item
@@ -61,10 +62,10 @@ struct Walk {
       set_error(a.err, kDevBadIndex);
       len = 0;
     }
-    tiles = (n * p->G + BM - 1) / BM;
+    tiles = (n * p->G + p->bm - 1) / p->bm;
   }
   __device__ __forceinline__ void tile(int tt) {
-    const int i0 = tt * BM / p->G, i1 = min(n - 1, (tt * BM + BM - 1) / p->G);
+    const int i0 = tt * p->bm / p->G, i1 = min(n - 1, (tt * p->bm + p->bm - 1) / p->G);
     hi = max(0, len - n + i1 + 1);
     lo = p->a.window > 0 ? max(0, len - n + i0 + 1 - p->a.window) : 0;
     blk0 = lo / BK;
@@ -101,22 +102,22 @@ struct Walk {
     if (more()) tile(t);
   }
   // keys [first, last) that row r of the tile sees
-  __device__ __forceinline__ int row_hi(int r) const { return len - n + (t * BM + r) / p->G + 1; }
+  __device__ __forceinline__ int row_hi(int r) const { return len - n + (t * p->bm + r) / p->G + 1; }
   __device__ __forceinline__ int row_lo(int r) const {
     return p->a.window > 0 ? max(0, row_hi(r) - p->a.window) : 0;
   }
-  __device__ __forceinline__ int rows() const { return min(BM, n * p->G - t * BM); }
+  __device__ __forceinline__ int rows() const { return min(p->bm, n * p->G - t * p->bm); }
 };
 
 // All NT threads of the CTA: the CTA's range of all blocks and its first item.  `total` and
 // `P` (CTAs that share the work) are the same in every CTA.
-template <int BM, int BK, int NT>
-__device__ __forceinline__ Walk<BM, BK> start_walk(const Params& p, int min_blocks, int64_t& total, int& P) {
+template <int BK, int NT>
+__device__ __forceinline__ Walk<BK> start_walk(const Params& p, int min_blocks, int64_t& total, int& P) {
   __shared__ int64_t warp_sum[NT / 32];
   __shared__ int64_t first_rem;
   __shared__ int first_seq;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  Walk<BM, BK> w;
+  Walk<BK> w;
   w.p = &p;
   const int per = (p.a.nseq + NT - 1) / NT;
   const int s0 = min(tid * per, p.a.nseq), s1 = min(s0 + per, p.a.nseq);
@@ -235,5 +236,7 @@ __device__ __noinline__ void row_attend(const Params& p, const int32_t* table, i
 
 int attn_paged_few(const paged::Params& p, cudaStream_t s);
 int64_t attn_paged_few_ctas();
+int attn_paged_many(const paged::Params& p, cudaStream_t s);
+int64_t attn_paged_many_ctas();
 
 }  // namespace rt

@@ -1009,6 +1009,18 @@ bool make_tmap_rows(CUtensorMap* tm, const void* ptr, uint64_t row_bytes, uint64
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_tmap_heads(CUtensorMap* tm, const void* ptr, uint64_t hd, uint64_t heads, uint64_t tokens, uint64_t ld,
+                     uint32_t box_heads, uint32_t box_tokens) {
+  if (!encoder_ready()) return false;
+  cuuint64_t dims[3] = {hd, heads, tokens};
+  cuuint64_t strides[2] = {hd * 2, ld * 2};
+  cuuint32_t box[3] = {64, box_heads, box_tokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int gemm_launch(const GemmArgs& g, cudaStream_t stream) {
   if (!encoder_ready()) return -2;
   if (g.M <= 0 || g.N <= 0 || g.K <= 0 || g.K % BK != 0 || g.N % 32 != 0) return -1;

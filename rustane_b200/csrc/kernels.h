@@ -71,6 +71,10 @@ bool make_tmap_bf16(CUtensorMap* tm, const void* ptr, uint64_t inner, uint64_t o
 // Contiguous rows of row_bytes, in boxes of box_bytes (64 or 128, swizzled by as much) x box_rows.
 bool make_tmap_rows(CUtensorMap* tm, const void* ptr, uint64_t row_bytes, uint64_t rows, uint32_t box_bytes,
                     uint32_t box_rows);
+// bf16 [tokens][heads][hd], token stride ld elements, in boxes of 64 columns x box_heads x box_tokens,
+// 128-byte swizzled.
+bool make_tmap_heads(CUtensorMap* tm, const void* ptr, uint64_t hd, uint64_t heads, uint64_t tokens, uint64_t ld,
+                     uint32_t box_heads, uint32_t box_tokens);
 int num_sms();
 // Floats a GemmArgs::sumsq buffer needs (8 per SM).
 int gemm_sumsq_slots();
