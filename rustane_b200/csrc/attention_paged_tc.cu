@@ -38,11 +38,11 @@ enum Bar : int {
   kVEmpty = 8,   // [2]
   kSFull = 10,   // [2]
   kSFree = 12,   // [2]
-  kPFull = 14,
-  kPvDone = 15,  // [2]
-  kOFree = 17,   // [2]
-  kDrain = 19,
-  kCodeFull = 20,                           // [kStages8]
+  kPFull = 14,   // [2] by S buffer: the softmax may finish block g + 1 before P of block g is waited for
+  kPvDone = 16,  // [2]
+  kOFree = 18,   // [2]
+  kDrain = 20,
+  kCodeFull = 21,                           // [kStages8]
   kCodeEmpty = kCodeFull + kStages8,        // [kStages8]
   kScaleFull = kCodeEmpty + kStages8,       // [kScaleSlots]
   kScaleEmpty = kScaleFull + kScaleSlots,   // [kScaleSlots]
@@ -99,8 +99,8 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
       mbar_init(&bar[kSFree + i], 1);
       mbar_init(&bar[kPvDone + i], 1);
       mbar_init(&bar[kOFree + i], 8);
+      mbar_init(&bar[kPFull + i], 8);
     }
-    mbar_init(&bar[kPFull], 8);
     mbar_init(&bar[kDrain], 1);
     for (int i = 0; i < kStages8; ++i) {
       mbar_init(&bar[kCodeFull + i], 1);
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
           fence_proxy_async_smem();
           __syncwarp();
         }
-        if (!wait(&bar[kPFull], g & 1) || (b == 0 && it >= 2 && !wait(&bar[kOFree + ob], ((it >> 1) - 1) & 1))) {
+        if (!wait(&bar[kPFull + st], (g >> 1) & 1) || (b == 0 && it >= 2 && !wait(&bar[kOFree + ob], ((it >> 1) - 1) & 1))) {
           ok = false;
           break;
         }
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&bar[kPFull]);
+          mbar_arrive(&bar[kPFull + st]);
           if (I8) mbar_arrive(&bar[kScaleEmpty + g % kScaleSlots]);
         }
       }

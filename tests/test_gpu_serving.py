@@ -398,6 +398,21 @@ def test_attention_long_contexts_split_and_joined(q_lens, kv_lens, H, Hk, int8):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])  # joined in a fixed order
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("n", [1, 500])
+def test_attention_with_cold_caches(n, int8):
+    """Slow K and V loads (L2 flushed before every call) shift the kernel's roles against one another: no
+    wait runs out, and the results are the same bits."""
+    p = Paged([n] * 3, [4000, 2500, n], 4, 2, 128, 16, int8, seed=21)
+    exp, exp_l = p.run()
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    for i in range(10):
+        flush.fill_(i)
+        got, lse = p.run()
+        assert torch.equal(got, exp) and torch.equal(lse, exp_l)
+    p.cache.check()
+
+
 @pytest.mark.parametrize("n", [1, 300])
 def test_attention_rising_scores(n):
     """Scores that grow along the keys force the running maximum up again and again."""
