@@ -26,8 +26,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
-constexpr int kSub = 16384;                // tokens counted at a time: 64 KB, three CTAs an SM
+constexpr int kThreads = 256;
+constexpr int kSub = 8192;                 // tokens counted at a time: 32 KB, four CTAs an SM
 constexpr uint32_t kSeen = 0x80000000u;    // occurs in the prompt part
 constexpr uint32_t kBiased = 0x40000000u;  // has a bias entry
 constexpr uint32_t kCount = 0x3fffffffu;
@@ -45,19 +45,26 @@ __device__ __forceinline__ Best better(Best a, Best b) {
 
 struct Params {
   LogitsArgs a;
-  int slice;  // tokens per CTA, a multiple of 128
+  int slice;  // places per CTA, a multiple of 128
 };
 
+constexpr int kBatch = 4;  // 16-byte loads (or 4-byte ones, VEC false) in flight per thread
+
+// VEC: the rows of in and out are equally far from a 16-byte boundary, so both take 16-byte
+// accesses from there on; place x = v + (that distance in floats) counts tokens from the
+// boundary before the row.  Otherwise x = v, 4 bytes at a time.
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads) logits_adjust_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const Params p) {
   extern __shared__ uint32_t cnt[];
   __shared__ Best warp_best[kThreads / 32];
-  __shared__ Best cta_best;
+  __shared__ Best cta_best[8];  // of the cluster's CTAs, in the first one
   const LogitsArgs& a = p.a;
   const int b = blockIdx.y, rank = blockIdx.x, tid = threadIdx.x;
-  const int lo_all = min(a.V, rank * p.slice), hi_all = min(a.V, lo_all + p.slice);
   const float* in = a.logits + b * a.ldl;
   float* out = a.out + b * a.ldo;
+  const int shift = VEC ? static_cast<int>((reinterpret_cast<uintptr_t>(in) >> 2) & 3) : 0;
+  const int x_end = a.V + shift;
+  const int lo_all = min(x_end, rank * p.slice), hi_all = min(x_end, lo_all + p.slice);
   auto clamp_to = [](int64_t v, int64_t n) { return v < 0 ? int64_t(0) : v > n ? n : v; };
   int64_t h0 = 0, h1 = 0, b0 = 0, b1 = 0;
   if (a.hist) {
@@ -84,79 +91,123 @@ __global__ void __launch_bounds__(kThreads) logits_adjust_kernel(const Params p)
   };
   auto allowed = [&](int v) { return !mask || ((mask[v >> 5] >> (v & 31)) & 1u); };
   auto consider = [&](float l, int v) {
-    if (l > best.v) best = {l, v};  // ascending v per thread within a pass: ties keep the first
+    if (l > best.v) best = {l, v};
     else if (l == best.v && best.i > v) best.i = v;
   };
 
+  // VEC: the thread's next kBatch vectors, one round ahead (the first are on their way while the
+  // history is counted); edge vectors of the row are read where they are used
+  constexpr int kRound = 4 * kThreads * kBatch;
+  float4 ahead[kBatch];
+  auto load = [&](int x0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int x = x0 + u * 4 * kThreads;
+      if (x >= shift && x + 4 <= x_end && x < hi_all) ahead[u] = __ldcs(reinterpret_cast<const float4*>(in + (x - shift)));
+    }
+  };
+  if (VEC) load(lo_all + 4 * tid);
+
   for (int lo = lo_all; lo < hi_all; lo += kSub) {
     const int hi = min(hi_all, lo + kSub), n = hi - lo;
+    const int id_lo = lo - shift, id_hi = hi - shift;  // tokens of these places
     if (counted) {
-      for (int i = tid; i < n; i += kThreads) cnt[i] = 0;
+      for (int i = 4 * tid; i < n; i += 4 * kThreads) *reinterpret_cast<uint4*>(cnt + i) = make_uint4(0, 0, 0, 0);
       __syncthreads();
-#pragma unroll 4
-      for (int64_t j = h0 + tid; j < h1; j += kThreads) {
-        const int id = a.hist[j];
-        if (id < 0 || id >= a.V) set_error(a.err, kDevBadToken);
-        else if (id >= lo && id < hi) {
-          if (j < made0) atomicOr(&cnt[id - lo], kSeen);
-          else atomicAdd(&cnt[id - lo], 1u);
+      for (int64_t j0 = h0 + tid; j0 < h1; j0 += kBatch * kThreads) {
+        int id[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) id[u] = j0 + u * kThreads < h1 ? a.hist[j0 + u * kThreads] : id_hi;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int64_t j = j0 + u * kThreads;
+          if (j < h1 && (id[u] < 0 || id[u] >= a.V)) set_error(a.err, kDevBadToken);
+          else if (id[u] >= id_lo && id[u] < id_hi && j < h1) {
+            if (j < made0) atomicOr(&cnt[id[u] - id_lo], kSeen);
+            else atomicAdd(&cnt[id[u] - id_lo], 1u);
+          }
         }
       }
       for (int64_t j = b0 + tid; j < b1; j += kThreads) {
         const int id = a.bias_ids[j];
         if (id < 0 || id >= a.V) set_error(a.err, kDevBadToken);
-        else if (id >= lo && id < hi) atomicOr(&cnt[id - lo], kBiased);
+        else if (id >= id_lo && id < id_hi) atomicOr(&cnt[id - id_lo], kBiased);
       }
       __syncthreads();
     }
     // A biased token's penalised logit waits in its count's place for the list below.
+    auto one = [&](int x, float raw) {
+      const int v = x - shift;
+      const uint32_t c = counted ? cnt[x - lo] : 0u;
+      float l = adjust(raw, c);
+      if (c & kBiased) {
+        cnt[x - lo] = __float_as_uint(l);
+        return;
+      }
+      if (!allowed(v)) l = -INFINITY;
+      consider(l, v);
+      __stcs(out + v, l);
+    };
     if (VEC) {
-#pragma unroll 2
-      for (int v = lo + 4 * tid; v < hi; v += 4 * kThreads) {
-        if (v + 4 <= hi) {
-          const float4 l4 = __ldcs(reinterpret_cast<const float4*>(in + v));
-          uint4 c4 = make_uint4(0, 0, 0, 0);
-          if (counted) c4 = *reinterpret_cast<const uint4*>(cnt + (v - lo));
-          const uint32_t bits = mask ? mask[v >> 5] >> (v & 31) : 0xfu;
-          float l[4] = {l4.x, l4.y, l4.z, l4.w};
-          const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+      for (int x0 = lo + 4 * tid; x0 < hi; x0 += kRound) {
+        float4 raw[kBatch];
+        uint32_t w0[kBatch], w1[kBatch];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            l[e] = adjust(l[e], c[e]);
-            if (c[e] & kBiased) {
-              cnt[v - lo + e] = __float_as_uint(l[e]);
-            } else {
-              if (!((bits >> e) & 1u)) l[e] = -INFINITY;
-              consider(l[e], v + e);
+        for (int u = 0; u < kBatch; ++u) {
+          const int x = x0 + u * 4 * kThreads, v = x - shift;
+          raw[u] = ahead[u];
+          w0[u] = w1[u] = ~0u;
+          if (mask && v >= 0 && x + 4 <= hi) {
+            w0[u] = mask[v >> 5];
+            w1[u] = mask[(v + 3) >> 5];
+          }
+        }
+        load(x0 + kRound < hi ? x0 + kRound : hi + 4 * tid);  // the next round, of this part or the next
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int x = x0 + u * 4 * kThreads, v = x - shift;
+          if (x >= hi) break;
+          if (v < 0 || x + 4 > x_end) {  // the row's first or last places
+            for (int y = max(x, shift); y < min(x + 4, hi); ++y) one(y, in[y - shift]);
+            continue;
+          }
+          float l[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+          uint4 c4 = make_uint4(0, 0, 0, 0);
+          if (counted) c4 = *reinterpret_cast<const uint4*>(cnt + (x - lo));
+          const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+          uint32_t bits = __funnelshift_r(w0[u], w1[u], v & 31);
+          if (c4.x | c4.y | c4.z | c4.w) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) l[e] = adjust(l[e], c[e]);
+            if ((c4.x | c4.y | c4.z | c4.w) & kBiased) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (c[e] & kBiased) {
+                  cnt[x - lo + e] = __float_as_uint(l[e]);
+                  bits &= ~(1u << e);  // not a candidate yet; the list writes it
+                }
             }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!((bits >> e) & 1u)) l[e] = -INFINITY;
+          // ascending order within a thread: only a larger value replaces the best
+          const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
+          if (top > best.v) {
+            best.v = top;
+            best.i = v + (l[0] == top ? 0 : l[1] == top ? 1 : l[2] == top ? 2 : 3);
           }
           __stcs(reinterpret_cast<float4*>(out + v), make_float4(l[0], l[1], l[2], l[3]));
-        } else {
-          for (int w = v; w < hi; ++w) {
-            const uint32_t c = counted ? cnt[w - lo] : 0u;
-            float l = adjust(in[w], c);
-            if (c & kBiased) {
-              cnt[w - lo] = __float_as_uint(l);
-              continue;
-            }
-            if (!allowed(w)) l = -INFINITY;
-            consider(l, w);
-            out[w] = l;
-          }
         }
       }
     } else {
-#pragma unroll 8
-      for (int v = lo + tid; v < hi; v += kThreads) {
-        const uint32_t c = counted ? cnt[v - lo] : 0u;
-        float l = adjust(__ldcs(in + v), c);
-        if (c & kBiased) {
-          cnt[v - lo] = __float_as_uint(l);
-        } else {
-          if (!allowed(v)) l = -INFINITY;
-          consider(l, v);
-          __stcs(out + v, l);
-        }
+      for (int x0 = lo + tid; x0 < hi; x0 += 2 * kBatch * kThreads) {
+        float raw[2 * kBatch];
+#pragma unroll
+        for (int u = 0; u < 2 * kBatch; ++u) raw[u] = x0 + u * kThreads < hi ? __ldcs(in + x0 + u * kThreads) : 0.f;
+#pragma unroll
+        for (int u = 0; u < 2 * kBatch; ++u)
+          if (x0 + u * kThreads < hi) one(x0 + u * kThreads, raw[u]);
       }
     }
     if (b1 > b0) {
@@ -170,24 +221,26 @@ __global__ void __launch_bounds__(kThreads) logits_adjust_kernel(const Params p)
           if (j < b1) {
             id = a.bias_ids[j];
             val = a.bias_vals[j];
-            if (id < lo || id >= hi) id = -1;
+            if (id < id_lo || id >= id_hi) id = -1;
           }
           const uint32_t same = __match_any_sync(0xffffffffu, id);
           const bool leader = id >= 0 && (same & ((1u << tid) - 1)) == 0;
-          float sum = leader ? __uint_as_float(cnt[id - lo]) : 0.f;
-          for (int k = 0; k < 32; ++k) {
-            const float other = __shfl_sync(0xffffffffu, val, k);
-            if (leader && ((same >> k) & 1u)) sum += other;
+          float sum = leader ? __uint_as_float(cnt[id - id_lo]) + val : 0.f;
+          if (__any_sync(0xffffffffu, id >= 0 && !leader)) {
+            for (int k = 0; k < 32; ++k) {
+              const float other = __shfl_sync(0xffffffffu, val, k);
+              if (leader && k != tid && ((same >> k) & 1u)) sum += other;
+            }
           }
-          if (leader) cnt[id - lo] = __float_as_uint(sum);
+          if (leader) cnt[id - id_lo] = __float_as_uint(sum);
           __syncwarp();
         }
       }
       __syncthreads();
       for (int64_t j = b0 + tid; j < b1; j += kThreads) {  // entries of one token write the same value
         const int id = a.bias_ids[j];
-        if (id < lo || id >= hi) continue;
-        float l = __uint_as_float(cnt[id - lo]);
+        if (id < id_lo || id >= id_hi) continue;
+        float l = __uint_as_float(cnt[id - id_lo]);
         if (!allowed(id)) l = -INFINITY;
         consider(l, id);
         out[id] = l;
@@ -202,17 +255,20 @@ __global__ void __launch_bounds__(kThreads) logits_adjust_kernel(const Params p)
     best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.i, o)});
   if ((tid & 31) == 0) warp_best[tid >> 5] = best;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kThreads / 32; ++w) best = better(best, warp_best[w]);
-    cta_best = best;
-  }
   cg::cluster_group cl = cg::this_cluster();
+  if (tid < 32) {
+    best = tid < kThreads / 32 ? warp_best[tid] : Best{-INFINITY, -1};
+#pragma unroll
+    for (int o = kThreads / 64; o; o >>= 1)
+      best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.i, o)});
+    if (tid == 0) *cl.map_shared_rank(&cta_best[rank], 0) = best;
+  }
   cl.sync();
   if (rank == 0 && tid == 0) {
-    for (int r = 1; r < static_cast<int>(gridDim.x); ++r) best = better(best, *cl.map_shared_rank(&cta_best, r));
+    best = cta_best[0];
+    for (int r = 1; r < static_cast<int>(gridDim.x); ++r) best = better(best, cta_best[r]);
     a.token[b] = best.i;
   }
-  cl.sync();  // no CTA leaves while its shared memory may be read
 }
 
 }  // namespace
@@ -225,13 +281,13 @@ int logits_adjust(const LogitsArgs& a, cudaStream_t s) {
   // once, but slices of 1024 tokens at least.
   const int sms = num_sms();
   int c = 1;
-  while (c < 8 && a.V / (2 * c) >= 1024 && (static_cast<int64_t>(a.B) * c < 2 * sms || a.V > c * kSub)) c *= 2;
+  while (c < 8 && a.V / (2 * c) >= 1024 && (static_cast<int64_t>(a.B) * c < 2 * sms || a.V > 2 * c * kSub)) c *= 2;
+  // VEC: equal distances from a 16-byte boundary in every row
+  const bool vec = (a.ldl - a.ldo) % 4 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.out)) & 15) == 0;
   Params p;
   p.a = a;
-  p.slice = ((a.V + c - 1) / c + 127) / 128 * 128;
-  // in and out rows on 16-byte boundaries take 16-byte accesses
-  const bool vec = a.ldl % 4 == 0 && a.ldo % 4 == 0 &&
-                   ((reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0;
+  p.slice = ((a.V + 3 + c - 1) / c + 127) / 128 * 128;
   const void* fn = vec ? reinterpret_cast<const void*>(logits_adjust_kernel<true>)
                        : reinterpret_cast<const void*>(logits_adjust_kernel<false>);
   const bool counted = a.hist || a.bias_ids;

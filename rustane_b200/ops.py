@@ -32,27 +32,27 @@ def _fail(msg: str):
     raise ValueError(msg)
 
 
-def _rows(name: str, t: torch.Tensor, cols: int, dtype: torch.dtype, device: torch.device, rows: int | None = None) -> None:
-    if t.dim() != 2 or t.dtype != dtype or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
-        _fail(f"{name}: expected a [{'T' if rows is None else rows}, {cols}] {dtype} tensor, got {tuple(t.shape)} {t.dtype}")
-    if t.device != device or (t.shape[0] and t.stride(1) != 1):
+def _rows(name: str, t: torch.Tensor, cols: int, dtype: torch.dtype, device: torch.device, rows: int | None = None) -> int:
+    """Checks a row matrix; its row stride, which torch leaves arbitrary where there are fewer than two rows."""
+    shape = t.shape
+    if len(shape) != 2 or t.dtype != dtype or shape[1] != cols or (rows is not None and shape[0] != rows):
+        _fail(f"{name}: expected a [{'T' if rows is None else rows}, {cols}] {dtype} tensor, got {tuple(shape)} {t.dtype}")
+    ld, step = t.stride()
+    if t.device != device or (shape[0] and step != 1):
         _fail(f"{name}: its rows have to be contiguous and on {device}")
+    return ld if shape[0] > 1 else max(ld, cols)
 
 
 def _vec(name: str, t: torch.Tensor, n: int | None, dtype: torch.dtype, device: torch.device) -> None:
-    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n):
-        _fail(f"{name}: expected {'a vector' if n is None else n} of {dtype}, got {tuple(t.shape)} {t.dtype}")
+    shape = t.shape
+    if t.dtype != dtype or len(shape) != 1 or (n is not None and shape[0] != n):
+        _fail(f"{name}: expected {'a vector' if n is None else n} of {dtype}, got {tuple(shape)} {t.dtype}")
     if t.device != device or not t.is_contiguous():
         _fail(f"{name}: has to be contiguous and on {device}")
 
 
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Row stride; torch leaves it arbitrary where there are fewer than two rows."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
 def _cuda(t: torch.Tensor) -> torch.device:
@@ -62,11 +62,14 @@ def _cuda(t: torch.Tensor) -> torch.device:
 
 
 def _call(name: str, device: torch.device, *args) -> None:
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            rc = getattr(lib(), name)(*args, torch.cuda.current_stream(device).cuda_stream)
+    # torch's raw handle of the current stream: the public Stream object costs 2 us to build, a
+    # tenth of a small call
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        rc = getattr(lib(), name)(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(device):
+            rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc != _lib.RT_OK:
         raise RustaneError(rc, name)
 
@@ -126,6 +129,7 @@ class KvCache:
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, device
         self.num_pages, self.kv_heads, self.page_size, self.hd = k.shape
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
+        self.err_ptr = self.err.data_ptr()
         self.c = RtKvPages(k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), self.num_pages, self.page_size,
                            self.kv_heads, self.hd, int(int8))
         self.ref = ctypes.byref(self.c)
@@ -152,6 +156,7 @@ class AttentionWorkspace:
     def __init__(self, device="cuda"):
         n = max(lib().rt_kernel_attention_paged_workspace_bytes(hd) for hd in (64, 128))
         self.buf = torch.zeros(n, dtype=torch.uint8, device=device)
+        self.ptr, self.size, self.device = self.buf.data_ptr(), n, self.buf.device
 
 
 def _gammas(gamma_q, gamma_k, hd, device):
@@ -180,15 +185,16 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, rope: Rope, heads: 
     device = _cuda(qkv)
     hd, nv = _vectors(qkv, heads, kv_heads)
     T, cols = qkv.shape
-    _rows("qkv", qkv, (heads + kv_heads + nv) * hd, torch.bfloat16, device)
+    ld = _rows("qkv", qkv, cols, torch.bfloat16, device)
     _vec("positions", positions, T, torch.int32, device)
     _gammas(gamma_q, gamma_k, hd, device)
     if rope.device != device:
         _fail(f"rope: its tables have to be on {device}")
     if out is None:
-        out = torch.empty((T, cols), dtype=torch.bfloat16, device=device)
-    _rows("out", out, cols, torch.bfloat16, device, T)
-    _call("rt_kernel_qk_norm_rope_fwd", device, qkv.data_ptr(), _ld(qkv), out.data_ptr(), _ld(out), positions.data_ptr(),
+        out, ldo = qkv.new_empty((T, cols)), cols
+    else:
+        ldo = _rows("out", out, cols, torch.bfloat16, device, T)
+    _call("rt_kernel_qk_norm_rope_fwd", device, qkv.data_ptr(), ld, out.data_ptr(), ldo, positions.data_ptr(),
           rope.ref, _ptr(gamma_q), _ptr(gamma_k), eps, T, heads, kv_heads, nv, hd, _ptr(err))
     return out
 
@@ -202,29 +208,30 @@ def qk_norm_rope_backward(dout: torch.Tensor, qkv: torch.Tensor | None, position
     device = _cuda(dout)
     hd, nv = _vectors(dout, heads, kv_heads)
     T, cols = dout.shape
-    _rows("dout", dout, (heads + kv_heads + nv) * hd, torch.bfloat16, device)
+    ld = _rows("dout", dout, cols, torch.bfloat16, device)
     _vec("positions", positions, T, torch.int32, device)
     _gammas(gamma_q, gamma_k, hd, device)
     if rope.device != device:
         _fail(f"rope: its tables have to be on {device}")
     if dqkv is None:
-        dqkv = torch.empty((T, cols), dtype=torch.bfloat16, device=device)
-    _rows("dqkv", dqkv, cols, torch.bfloat16, device, T)
-    accumulate, partials = 0, None
+        dqkv, lddx = dout.new_empty((T, cols)), cols
+    else:
+        lddx = _rows("dqkv", dqkv, cols, torch.bfloat16, device, T)
+    accumulate, partials, ldx = 0, None, 0
     if gamma_q is not None:
         if qkv is None:
             _fail("the gammas' backward reads qkv")
-        _rows("qkv", qkv, cols, torch.bfloat16, device, T)
+        ldx = _rows("qkv", qkv, cols, torch.bfloat16, device, T)
         if (dgamma_q is None) != (dgamma_k is None):
             _fail("dgamma_q and dgamma_k: both or neither")
         accumulate = int(dgamma_q is not None)
-        if not accumulate:
-            dgamma_q, dgamma_k = torch.empty((2, hd), device=device).unbind(0)
-        _vec("dgamma_q", dgamma_q, hd, torch.float32, device)
-        _vec("dgamma_k", dgamma_k, hd, torch.float32, device)
-        partials = torch.empty(lib().rt_kernel_qk_norm_rope_bwd_partials(T, heads, kv_heads) * hd, device=device)
-    _call("rt_kernel_qk_norm_rope_bwd", device, dout.data_ptr(), _ld(dout), _ptr(qkv), _ld(qkv) if qkv is not None else 0,
-          dqkv.data_ptr(), _ld(dqkv), positions.data_ptr(), rope.ref, _ptr(gamma_q), _ptr(gamma_k), eps, _ptr(dgamma_q),
+        if accumulate:
+            _vec("dgamma_q", dgamma_q, hd, torch.float32, device)
+            _vec("dgamma_k", dgamma_k, hd, torch.float32, device)
+        else:
+            dgamma_q, dgamma_k = torch.empty_like(gamma_q), torch.empty_like(gamma_k)
+        partials = gamma_q.new_empty(lib().rt_kernel_qk_norm_rope_bwd_partials(T, heads, kv_heads) * hd)
+    _call("rt_kernel_qk_norm_rope_bwd", device, dout.data_ptr(), ld, _ptr(qkv), ldx, dqkv.data_ptr(), lddx, positions.data_ptr(), rope.ref, _ptr(gamma_q), _ptr(gamma_k), eps, _ptr(dgamma_q),
           _ptr(dgamma_k), accumulate, _ptr(partials), T, heads, kv_heads, nv, hd, _ptr(err))
     return dqkv, dgamma_q, dgamma_k
 
@@ -235,17 +242,18 @@ def kv_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, r
     """qk_norm_rope that writes k and v of token t into cache slot slots[t] (-1: nowhere) and returns q."""
     device = cache.device
     T, hd = qkv.shape[0], cache.hd
-    _rows("qkv", qkv, (heads + 2 * cache.kv_heads) * hd, torch.bfloat16, device)
+    ld = _rows("qkv", qkv, (heads + 2 * cache.kv_heads) * hd, torch.bfloat16, device)
     _vec("positions", positions, T, torch.int32, device)
     _vec("slots", slots, T, torch.int32, device)
     _gammas(gamma_q, gamma_k, hd, device)
     if rope.device != device:
         _fail(f"rope: its tables have to be on {device}")
     if q_out is None:
-        q_out = torch.empty((T, heads * hd), dtype=torch.bfloat16, device=device)
-    _rows("q_out", q_out, heads * hd, torch.bfloat16, device, T)
-    _call("rt_kernel_kv_append", device, qkv.data_ptr(), _ld(qkv), q_out.data_ptr(), _ld(q_out), positions.data_ptr(),
-          slots.data_ptr(), rope.ref, _ptr(gamma_q), _ptr(gamma_k), eps, cache.ref, T, heads, cache.err.data_ptr())
+        q_out, ldq = qkv.new_empty((T, heads * hd)), heads * hd
+    else:
+        ldq = _rows("q_out", q_out, heads * hd, torch.bfloat16, device, T)
+    _call("rt_kernel_kv_append", device, qkv.data_ptr(), ld, q_out.data_ptr(), ldq, positions.data_ptr(),
+          slots.data_ptr(), rope.ref, _ptr(gamma_q), _ptr(gamma_k), eps, cache.ref, T, heads, cache.err_ptr)
     return q_out
 
 
@@ -255,13 +263,14 @@ def kv_gather(cache: KvCache, slots: torch.Tensor, k_out: torch.Tensor | None = 
     device, T = cache.device, slots.shape[0]
     _vec("slots", slots, T, torch.int32, device)
     shape = (T, cache.kv_heads, cache.hd)
+    given = [x for x in (("k_out", k_out), ("v_out", v_out)) if x[1] is not None]
     k_out = torch.empty(shape, dtype=torch.bfloat16, device=device) if k_out is None else k_out
-    v_out = torch.empty(shape, dtype=torch.bfloat16, device=device) if v_out is None else v_out
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
+    v_out = torch.empty_like(k_out) if v_out is None else v_out
+    for name, t in given:
         if t.shape != shape or t.dtype != torch.bfloat16 or t.device != device or not t.is_contiguous():
             _fail(f"{name}: a contiguous bf16 {shape} tensor on {device}")
     _call("rt_kernel_kv_gather", device, cache.ref, slots.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
-          cache.kv_heads * cache.hd, T, cache.err.data_ptr())
+          cache.kv_heads * cache.hd, T, cache.err_ptr)
     return k_out, v_out
 
 
@@ -274,20 +283,21 @@ def attention_paged(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, k
     Returns (out [T, heads * hd] bf16, lse2 [T, heads] fp32 or None)."""
     device, T, n = cache.device, q.shape[0], kv_lens.shape[0]
     cols = heads * cache.hd
-    _rows("q", q, cols, torch.bfloat16, device)
+    ldq = _rows("q", q, cols, torch.bfloat16, device)
     _vec("kv_lens", kv_lens, n, torch.int32, device)
     _vec("q_start", q_start, n + 1, torch.int32, device)
-    _rows("page_table", page_table, page_table.shape[1] if page_table.dim() == 2 else 0, torch.int32, device, n)
+    ldt = _rows("page_table", page_table, page_table.shape[-1], torch.int32, device, n)
     if out is None:
-        out = torch.empty((T, cols), dtype=torch.bfloat16, device=device)
-    _rows("out", out, cols, torch.bfloat16, device, T)
-    if workspace.buf.device != device:
+        out, ldo = q.new_empty((T, cols)), cols
+    else:
+        ldo = _rows("out", out, cols, torch.bfloat16, device, T)
+    if workspace.device != device:
         _fail(f"workspace: has to be on {device}")
     lse2 = torch.empty((T, heads), device=device) if want_lse else None
-    _call("rt_kernel_attention_paged", device, q.data_ptr(), _ld(q), out.data_ptr(), _ld(out), _ptr(lse2), cache.ref,
-          page_table.data_ptr(), _ld(page_table), kv_lens.data_ptr(), q_start.data_ptr(), n, T, max_q, max_kv, heads, window,
-          1.0 / math.sqrt(cache.hd) if scale is None else scale, workspace.buf.data_ptr(), workspace.buf.numel(),
-          cache.err.data_ptr())
+    _call("rt_kernel_attention_paged", device, q.data_ptr(), ldq, out.data_ptr(), ldo, _ptr(lse2), cache.ref,
+          page_table.data_ptr(), ldt, kv_lens.data_ptr(), q_start.data_ptr(), n, T, max_q, max_kv, heads, window,
+          1.0 / math.sqrt(cache.hd) if scale is None else scale, workspace.ptr, workspace.size,
+          cache.err_ptr)
     return out, lse2
 
 
@@ -304,7 +314,7 @@ def logits_adjust(logits: torch.Tensor, hist: torch.Tensor | None = None, hist_s
     if logits.dim() != 2:
         _fail("logits: [B, V]")
     B, V = logits.shape
-    _rows("logits", logits, V, torch.float32, device)
+    ldl = _rows("logits", logits, V, torch.float32, device)
     r = RtLogitRules()
     if hist is not None:
         if hist_start is None:
@@ -328,12 +338,13 @@ def logits_adjust(logits: torch.Tensor, hist: torch.Tensor | None = None, hist_s
         r.bias_ids, r.bias_vals, r.bias_start, r.n_bias = (bias_ids.data_ptr(), bias_vals.data_ptr(), bias_start.data_ptr(),
                                                            bias_ids.shape[0])
     if mask is not None:
-        _rows("mask", mask, (V + 31) // 32, torch.int32, device, B)
-        r.mask, r.mask_ld = mask.data_ptr(), _ld(mask)
+        r.mask_ld = _rows("mask", mask, (V + 31) // 32, torch.int32, device, B)
+        r.mask = mask.data_ptr()
     if out is None:
-        out = torch.empty((B, V), device=device)
-    _rows("out", out, V, torch.float32, device, B)
+        out, ldo = logits.new_empty((B, V)), V
+    else:
+        ldo = _rows("out", out, V, torch.float32, device, B)
     token = torch.empty(B, dtype=torch.int32, device=device)
-    _call("rt_kernel_logits_adjust", device, logits.data_ptr(), _ld(logits), out.data_ptr(), _ld(out), token.data_ptr(), B, V,
+    _call("rt_kernel_logits_adjust", device, logits.data_ptr(), ldl, out.data_ptr(), ldo, token.data_ptr(), B, V,
           ctypes.byref(r), _ptr(err))
     return out, token
