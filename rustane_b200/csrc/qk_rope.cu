@@ -12,10 +12,14 @@
 // the nearest one), read back as code * s.  A row with a NaN or infinity gets a
 // NaN scale and reads back as NaN.  All arithmetic in fp32, rounded once.
 //
-// All are HBM-bound.  hd / 8 lanes own one head vector, 16 bytes a lane, so a
-// warp holds 32 / (hd / 8) vectors; a warp takes kU such groups of one token
-// at a time, loads first, so kU 512-byte loads are in flight, and the token's
-// tables and the gammas are read once per kU groups.
+// All are HBM-bound.  hd / 8 lanes own one head vector: a lane holds 4 first entries of
+// rotated pairs and their 4 second ones (interleaved: 16 contiguous bytes; halves: 8 bytes each
+// of two places), so pairs never cross lanes, and all arithmetic runs in packed fp32x2.  A
+// warp holds 32 / (hd / 8) vectors; kU (backward kUb) of these are a group, loaded at once.
+// The groups of all tokens are cut into equal runs, one per warp of a grid that fits the
+// GPU: a warp has the next group's loads in flight while it works on one, and reads a token's
+// position and tables once per run.  (Pairs exchanged by shuffles and scalar arithmetic: 17
+// instructions an entry, half of all issue slots, 4.2 TB/s on 8209 tokens of 96 heads.)
 #include "common.cuh"
 #include "kernels.h"
 #include "serving.h"
@@ -25,33 +29,23 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kU = 4;
+constexpr int kCtasPerSm = 2;
+constexpr int kU = 4;   // vectors per lane group and group of heads: forward, gather
+constexpr int kUb = 2;  // backward, which holds two inputs and two running sums
 
-__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
-  v[0] = bf16lo(u.x); v[1] = bf16hi(u.x); v[2] = bf16lo(u.y); v[3] = bf16hi(u.y);
-  v[4] = bf16lo(u.z); v[5] = bf16hi(u.z); v[6] = bf16lo(u.w); v[7] = bf16hi(u.w);
-}
-__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
-  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                    pack_bf16x2(v[6], v[7]));
-}
-__device__ __forceinline__ void load8f(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
-// Sum / max over the LPH lanes that share a head vector.
+// Sum / max over the LPH lanes that share a head vector (`mask`: at least those lanes).
 template <int LPH>
-__device__ __forceinline__ float head_sum(float v) {
+__device__ __forceinline__ float head_sum(float v, uint32_t mask) {
 #pragma unroll
-  for (int o = LPH / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = LPH / 2; o; o >>= 1) v += __shfl_xor_sync(mask, v, o);
   return v;
 }
 template <int LPH>
-__device__ __forceinline__ float head_max(float v) {
+__device__ __forceinline__ float head_max(float v, uint32_t mask) {
 #pragma unroll
-  for (int o = LPH / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = LPH / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
   return v;
 }
 
@@ -59,51 +53,123 @@ struct RopeDev {
   const float* cos;
   const float* sin;
   const int32_t* pos;
-  int n_pos, rot, half;
+  int n_pos, rot;
 };
 
-// One lane's part of a token's tables: interleaved pairs need 4 angles, halves 8.
+// Where lane `sub` of a vector finds its entries: 4 at a, 4 at b (interleaved: a's 8 entries
+// alternate between the two).  Lanes past the rotated columns take 8 contiguous ones.
+template <bool HALF>
+struct Place {
+  int a, b;
+  bool turns;
+  __device__ __forceinline__ Place(int sub, int rot) {
+    turns = sub * 8 < rot;
+    a = HALF && turns ? sub * 4 : sub * 8;
+    b = HALF && turns ? sub * 4 + rot / 2 : sub * 8 + 4;
+  }
+  // the 8 entries as packed pairs of first entries f[2] and of second ones s[2]
+  __device__ __forceinline__ void unpack(const uint4& u, uint64_t (&f)[2], uint64_t (&s)[2]) const {
+    if (HALF) {
+      f[0] = f2_pack(bf16lo(u.x), bf16hi(u.x));
+      f[1] = f2_pack(bf16lo(u.y), bf16hi(u.y));
+      s[0] = f2_pack(bf16lo(u.z), bf16hi(u.z));
+      s[1] = f2_pack(bf16lo(u.w), bf16hi(u.w));
+    } else {
+      f[0] = f2_pack(bf16lo(u.x), bf16lo(u.y));
+      f[1] = f2_pack(bf16lo(u.z), bf16lo(u.w));
+      s[0] = f2_pack(bf16hi(u.x), bf16hi(u.y));
+      s[1] = f2_pack(bf16hi(u.z), bf16hi(u.w));
+    }
+  }
+  // v[8] in the order of the entries at a, then at b
+  __device__ __forceinline__ void spread(const uint64_t (&f)[2], const uint64_t (&s)[2], float (&v)[8]) const {
+    if (HALF) {
+      f2_unpack(f[0], v[0], v[1]);
+      f2_unpack(f[1], v[2], v[3]);
+      f2_unpack(s[0], v[4], v[5]);
+      f2_unpack(s[1], v[6], v[7]);
+    } else {
+      f2_unpack(f[0], v[0], v[2]);
+      f2_unpack(f[1], v[4], v[6]);
+      f2_unpack(s[0], v[1], v[3]);
+      f2_unpack(s[1], v[5], v[7]);
+    }
+  }
+  __device__ __forceinline__ uint4 load(const __nv_bfloat16* row) const {
+    if (!HALF) return *reinterpret_cast<const uint4*>(row + a);
+    const uint2 x = *reinterpret_cast<const uint2*>(row + a), y = *reinterpret_cast<const uint2*>(row + b);
+    return make_uint4(x.x, x.y, y.x, y.y);
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* row, const uint4& u) const {
+    if (HALF) {
+      *reinterpret_cast<uint2*>(row + a) = make_uint2(u.x, u.y);
+      *reinterpret_cast<uint2*>(row + b) = make_uint2(u.z, u.w);
+    } else {
+      *reinterpret_cast<uint4*>(row + a) = u;
+    }
+  }
+  __device__ __forceinline__ uint4 pack(const uint64_t (&f)[2], const uint64_t (&s)[2]) const {
+    float v[8];
+    spread(f, s, v);
+    return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                      pack_bf16x2(v[6], v[7]));
+  }
+  // the lane's entries of an fp32 vector, in the same packing
+  __device__ __forceinline__ void gather(const float* g, uint64_t (&f)[2], uint64_t (&s)[2]) const {
+    const float4 x = load4(g + a), y = load4(g + b);
+    if (HALF) {
+      f[0] = f2_pack(x.x, x.y);
+      f[1] = f2_pack(x.z, x.w);
+      s[0] = f2_pack(y.x, y.y);
+      s[1] = f2_pack(y.z, y.w);
+    } else {
+      f[0] = f2_pack(x.x, x.z);
+      f[1] = f2_pack(y.x, y.z);
+      s[0] = f2_pack(x.y, x.w);
+      s[1] = f2_pack(y.y, y.w);
+    }
+  }
+};
+
+// One lane's 4 angles of a token (either layout: pairs 4 sub .. 4 sub + 3).
 struct Angles {
-  float c[8], s[8];
+  uint64_t c[2], s[2];
 };
 __device__ __forceinline__ void load_angles(Angles& a, const RopeDev& r, int pos, int sub) {
-  const int d0 = sub * 8;
-  if (d0 >= r.rot) return;
-  const int64_t base = static_cast<int64_t>(pos) * (r.rot / 2);
-  if (r.half) {
-    const int i = d0 < r.rot / 2 ? d0 : d0 - r.rot / 2;
-    load8f(r.cos + base + i, a.c);
-    load8f(r.sin + base + i, a.s);
-  } else {
-    const float4 c = *reinterpret_cast<const float4*>(r.cos + base + d0 / 2);
-    const float4 s = *reinterpret_cast<const float4*>(r.sin + base + d0 / 2);
-    a.c[0] = c.x; a.c[1] = c.y; a.c[2] = c.z; a.c[3] = c.w;
-    a.s[0] = s.x; a.s[1] = s.y; a.s[2] = s.z; a.s[3] = s.w;
+  const int64_t at = static_cast<int64_t>(pos) * (r.rot / 2) + sub * 4;
+  const float4 c = load4(r.cos + at), s = load4(r.sin + at);
+  a.c[0] = f2_pack(c.x, c.y);
+  a.c[1] = f2_pack(c.z, c.w);
+  a.s[0] = f2_pack(s.x, s.y);
+  a.s[1] = f2_pack(s.z, s.w);
+}
+__device__ __forceinline__ uint64_t f2_neg(uint64_t x) { return x ^ 0x8000000080000000ull; }
+// (f, s) <- R (f, s) (BACK: R^T)
+template <bool BACK>
+__device__ __forceinline__ void rotate(uint64_t (&f)[2], uint64_t (&s)[2], const Angles& a) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t up = BACK ? a.s[i] : f2_neg(a.s[i]), dn = BACK ? f2_neg(a.s[i]) : a.s[i];
+    const uint64_t x = f2_fma(s[i], up, f2_mul(f[i], a.c[i]));
+    s[i] = f2_fma(f[i], dn, f2_mul(s[i], a.c[i]));
+    f[i] = x;
   }
 }
-// v <- R v (BACK: R^T v).  Every lane of the warp calls it (the halves exchange by shuffles).
-template <int LPH, bool BACK>
-__device__ __forceinline__ void rotate(float (&v)[8], const Angles& a, const RopeDev& r, int sub) {
-  const int d0 = sub * 8;
-  if (r.half) {
-    const int step = r.rot / 16;  // lanes between the two halves of a pair
-    const bool first = d0 < r.rot / 2;
-    const int lane = threadIdx.x & 31;
-    const int src = d0 >= r.rot ? lane : first ? lane + step : lane - step;
+// (f, s) <- (f, s) * r * (g, h)
+__device__ __forceinline__ void scale(uint64_t (&f)[2], uint64_t (&s)[2], float r, const uint64_t (&g)[2],
+                                      const uint64_t (&h)[2]) {
+  const uint64_t r2 = f2_pack(r, r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float p = __shfl_sync(0xffffffffu, v[i], src);
-      const float s = first != BACK ? -a.s[i] : a.s[i];
-      if (d0 < r.rot) v[i] = v[i] * a.c[i] + p * s;
-    }
-  } else if (d0 < r.rot) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = v[2 * i], y = v[2 * i + 1], s = BACK ? -a.s[i] : a.s[i];
-      v[2 * i] = x * a.c[i] - y * s;
-      v[2 * i + 1] = y * a.c[i] + x * s;
-    }
+  for (int i = 0; i < 2; ++i) {
+    f[i] = f2_mul(f2_mul(f[i], r2), g[i]);
+    s[i] = f2_mul(f2_mul(s[i], r2), h[i]);
   }
+}
+__device__ __forceinline__ float dot8(const uint64_t (&f)[2], const uint64_t (&s)[2], const uint64_t (&g)[2],
+                                      const uint64_t (&h)[2]) {
+  float x, y;
+  f2_unpack(f2_fma(s[1], h[1], f2_fma(s[0], h[0], f2_fma(f[1], g[1], f2_mul(f[0], g[0])))), x, y);
+  return x + y;
 }
 
 struct FwdParams {
@@ -128,107 +194,177 @@ struct FwdParams {
 
 enum Dest : int { kToRows, kToBf16Pages, kToInt8Pages };
 
-template <int HD, int DEST>
-__global__ void __launch_bounds__(kThreads) qk_rope_fwd_kernel(const FwdParams p) {
+// A warp's run [g, g1) of the groups (token, chunk of heads), and the position at hand.
+struct Run {
+  int64_t g, g1;
+  int tok, chunk;
+  __device__ __forceinline__ Run(int64_t groups, int chunks) {
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    const int64_t n = static_cast<int64_t>(gridDim.x) * kWarps;
+    g = groups * w / n;
+    g1 = groups * (w + 1) / n;
+    tok = static_cast<int>(g / chunks);
+    chunk = static_cast<int>(g - static_cast<int64_t>(tok) * chunks);
+  }
+  __device__ __forceinline__ void next(int chunks) {
+    ++g;
+    if (++chunk == chunks) {
+      chunk = 0;
+      ++tok;
+    }
+  }
+};
+
+__device__ __forceinline__ int position(const RopeDev& r, int tok, int* err) {
+  const int pos = r.pos[tok];
+  if (pos >= 0 && pos < r.n_pos) return pos;
+  set_error(err, kDevBadIndex);
+  return 0;
+}
+
+template <int HD, int DEST, bool HALF>
+__global__ void __launch_bounds__(kThreads, 2) qk_rope_fwd_kernel(const FwdParams p) {
   constexpr int LPH = HD / 8, HPW = 32 / LPH;  // lanes per head vector, vectors per warp
+  __shared__ __align__(16) float gam[2][HD];
   const int lane = threadIdx.x & 31, sub = lane % LPH, hw = lane / LPH;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t tok64 = item / p.chunks;
-  if (tok64 >= p.T) return;  // the whole warp
-  const int tok = static_cast<int>(tok64);
-  const int h0 = static_cast<int>(item - tok64 * p.chunks) * (HPW * kU) + hw;
-
-  uint4 raw[kU];
-  const __nv_bfloat16* row = p.x + tok * p.ldx + sub * 8;
+  const uint32_t mates = ((1u << LPH) - 1u) << (hw * LPH);  // the vector's lanes
+  const Place<HALF> at(sub, p.rope.rot);
+  if (p.gq) {
+    for (int i = threadIdx.x; i < 2 * HD; i += kThreads) gam[i / HD][i % HD] = (i < HD ? p.gq : p.gk)[i % HD];
+    __syncthreads();
+  }
+  Run run(static_cast<int64_t>(p.T) * p.chunks, p.chunks);
+  uint4 ahead[kU];
+  auto load = [&](const Run& r) {
+    const __nv_bfloat16* row = p.x + r.tok * p.ldx;
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    const int h = h0 + u * HPW;
-    raw[u] = h < p.total_heads ? *reinterpret_cast<const uint4*>(row + static_cast<int64_t>(h) * HD)
-                               : make_uint4(0, 0, 0, 0);
-  }
-  int pos = p.rope.pos[tok];
-  if (pos < 0 || pos >= p.rope.n_pos) {
-    if (lane == 0) set_error(p.err, kDevBadIndex);
-    pos = 0;
-  }
-  int64_t slot = -1;
-  if (DEST != kToRows) {
-    slot = p.slots[tok];
-    if (slot < -1 || slot >= p.n_slots) {
-      if (lane == 0) set_error(p.err, kDevBadIndex);
-      slot = -1;
+    for (int u = 0; u < kU; ++u) {
+      const int h = r.chunk * (HPW * kU) + hw + u * HPW;
+      ahead[u] = make_uint4(0, 0, 0, 0);
+      if (r.g < r.g1 && h < p.total_heads) ahead[u] = at.load(row + static_cast<int64_t>(h) * HD);
     }
-  }
+  };
+  load(run);
   Angles ang;
-  load_angles(ang, p.rope, pos, sub);
+  int64_t slot = -1;
+  int have = -1;  // the token whose angles and slot are at hand
+  while (run.g < run.g1) {
+    const int tok = run.tok, run_chunk = run.chunk, h0 = run_chunk * (HPW * kU) + hw;
+    if (tok != have) {
+      const int pos = position(p.rope, tok, p.err);
+      if (at.turns) load_angles(ang, p.rope, pos, sub);
+      if (DEST != kToRows) {
+        slot = p.slots[tok];
+        if (slot < -1 || slot >= p.n_slots) {
+          set_error(p.err, kDevBadIndex);
+          slot = -1;
+        }
+      }
+      have = tok;
+    }
+    uint4 raw[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) raw[u] = ahead[u];
+    run.next(p.chunks);
+    load(run);
+
+    const int h_first = run_chunk * (HPW * kU), h_last = h_first + HPW * kU - 1;
+    const bool all_turn = h_last < p.heads + p.kv_heads;  // the group holds q and k vectors only
+    uint64_t f[kU][2], s[kU][2];
+    if (all_turn || DEST == kToInt8Pages || h_first < p.heads + p.kv_heads) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) at.unpack(raw[u], f[u], s[u]);
+    }
+    // Of a group of q and k vectors alone the kU chains of loads, sums and shuffles run side by
+    // side; a mixed group takes them one by one.
+    if (all_turn) {
+      float r[kU];
+      if (p.gq) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) r[u] = dot8(f[u], s[u], f[u], s[u]);
+#pragma unroll
+        for (int o = LPH / 2; o; o >>= 1)
+#pragma unroll
+          for (int u = 0; u < kU; ++u) r[u] += __shfl_xor_sync(0xffffffffu, r[u], o);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          uint64_t gf[2], gs[2];
+          at.gather(gam[h0 + u * HPW < p.heads ? 0 : 1], gf, gs);
+          scale(f[u], s[u], rsqrtf(r[u] * (1.0f / HD) + p.eps), gf, gs);
+        }
+      }
+      if (at.turns) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) rotate<false>(f[u], s[u], ang);
+      }
+#pragma unroll
+      for (int u = 0; u < kU; ++u) raw[u] = at.pack(f[u], s[u]);
+    } else if (h_first < p.heads + p.kv_heads) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int h = h0 + u * HPW;
+        if (h >= p.heads + p.kv_heads) continue;  // a whole vector's lanes
+        if (p.gq) {
+          uint64_t gf[2], gs[2];
+          at.gather(gam[h < p.heads ? 0 : 1], gf, gs);
+          scale(f[u], s[u], rsqrtf(head_sum<LPH>(dot8(f[u], s[u], f[u], s[u]), mates) * (1.0f / HD) + p.eps), gf, gs);
+        }
+        if (at.turns) rotate<false>(f[u], s[u], ang);
+        raw[u] = at.pack(f[u], s[u]);
+      }
+    }
 
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    const int h = h0 + u * HPW;
-    const bool is_q = h < p.heads, is_v = h >= p.heads + p.kv_heads;
-    float v[8];
-    unpack8(raw[u], v);
-    if (p.gq) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
-      const float r = rsqrtf(head_sum<LPH>(ss) * (1.0f / HD) + p.eps);
-      if (!is_v) {
-        float g[8];
-        load8f((is_q ? p.gq : p.gk) + sub * 8, g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * r * g[i];
+    for (int u = 0; u < kU; ++u) {
+      const int h = h0 + u * HPW;
+      if (h >= p.total_heads) continue;
+      const bool is_q = h < p.heads, is_v = h >= p.heads + p.kv_heads;
+      if (DEST == kToRows || is_q) {
+        at.store(p.out + tok * p.ldo + static_cast<int64_t>(h) * HD, raw[u]);
+        continue;
       }
-    }
-    float w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = v[i];
-    rotate<LPH, false>(w, ang, p.rope, sub);
-    if (!is_v) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = w[i];
-    }
-    float amax = 0.f;
-    bool finite = true;
-    if (DEST == kToInt8Pages) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        amax = fmaxf(amax, fabsf(v[i]));
-        finite = finite && isfinite(v[i]);
-      }
-      amax = head_max<LPH>(finite ? amax : INFINITY);
-    }
-    if (h >= p.total_heads) continue;
-    if (DEST == kToRows || is_q) {
-      *reinterpret_cast<uint4*>(p.out + tok * p.ldo + static_cast<int64_t>(h) * HD + sub * 8) = pack8(v);
-    } else if (slot >= 0) {
       const int kh = is_v ? h - p.heads - p.kv_heads : h - p.heads;
       const int64_t page = slot >> p.page_shift, off = slot & ((1 << p.page_shift) - 1);
-      const int64_t at = (((page * p.kv_heads + kh) << p.page_shift) + off);
+      const int64_t row = (((page * p.kv_heads + kh) << p.page_shift) + off);
       if (DEST == kToBf16Pages) {
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(is_v ? p.cv : p.ck) + at * HD + sub * 8) = pack8(v);
+        if (slot >= 0) at.store(static_cast<__nv_bfloat16*>(is_v ? p.cv : p.ck) + row * HD, raw[u]);
       } else {
-        const float s = isinf(amax) ? NAN : amax / 127.0f;
+        float v[8], amax = 0.f;
+        at.spread(f[u], s[u], v);
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          amax = fmaxf(amax, fabsf(v[i]));
+          finite = finite && isfinite(v[i]);
+        }
+        amax = head_max<LPH>(finite ? amax : INFINITY, mates);
+        const float scale = isinf(amax) ? NAN : amax / 127.0f;
         uint32_t b[2] = {0, 0};
-        if (s > 0.f) {
+        if (scale > 0.f) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             // |y / s| <= 127 but for the rounding of a denormal scale
-            const int c = max(-127, min(127, __float2int_rn(v[i] / s)));
+            const int c = max(-127, min(127, __float2int_rn(v[i] / scale)));
             b[i >> 2] |= static_cast<uint32_t>(c & 0xff) << (8 * (i & 3));
           }
         }
-        *reinterpret_cast<uint2*>(static_cast<int8_t*>(is_v ? p.cv : p.ck) + at * HD + sub * 8) =
-            make_uint2(b[0], b[1]);
-        if (sub == 0) (is_v ? p.sv : p.sk)[at] = s;
+        if (slot >= 0) {
+          int8_t* dst = static_cast<int8_t*>(is_v ? p.cv : p.ck) + row * HD;
+          if (HALF) {
+            *reinterpret_cast<uint32_t*>(dst + at.a) = b[0];
+            *reinterpret_cast<uint32_t*>(dst + at.b) = b[1];
+          } else {
+            *reinterpret_cast<uint2*>(dst + at.a) = make_uint2(b[0], b[1]);
+          }
+          if (sub == 0) (is_v ? p.sv : p.sk)[row] = scale;
+        }
       }
     }
   }
 }
 
-// Backward.  A fixed grid walks the items (token, kU groups of heads) in strides, so
-// every warp keeps its dgamma sums in registers; each CTA adds its warps' sums in a
-// fixed order and writes one partial row per gamma.
+// Backward.  Every warp keeps the dgamma sums of its run in registers; each CTA adds its
+// warps' sums in a fixed order and writes one partial row per gamma.
 struct BwdParams {
   const __nv_bfloat16* dy;
   int64_t lddy;
@@ -245,78 +381,127 @@ struct BwdParams {
   int* err;
 };
 
-template <int HD>
-__global__ void __launch_bounds__(kThreads) qk_rope_bwd_kernel(const BwdParams p) {
+template <int HD, bool HALF>
+__global__ void __launch_bounds__(kThreads, 2) qk_rope_bwd_kernel(const BwdParams p) {
   constexpr int LPH = HD / 8, HPW = 32 / LPH;
   __shared__ float red[2][kWarps * HPW][HD];
+  __shared__ __align__(16) float gam[2][HD];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LPH, hw = lane / LPH;
-  const int64_t items = static_cast<int64_t>(p.T) * p.chunks;
-  float gq[8], gk[8], dgq[8], dgk[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) gq[i] = gk[i] = dgq[i] = dgk[i] = 0.f;
+  const uint32_t mates = ((1u << LPH) - 1u) << (hw * LPH);
+  const Place<HALF> at(sub, p.rope.rot);
   if (p.gq) {
-    load8f(p.gq + sub * 8, gq);
-    load8f(p.gk + sub * 8, gk);
+    for (int i = threadIdx.x; i < 2 * HD; i += kThreads) gam[i / HD][i % HD] = (i < HD ? p.gq : p.gk)[i % HD];
+    __syncthreads();
   }
-  for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + warp; item < items;
-       item += static_cast<int64_t>(gridDim.x) * kWarps) {
-    const int64_t tok = item / p.chunks;
-    const int h0 = static_cast<int>(item - tok * p.chunks) * (HPW * kU) + hw;
-    uint4 rd[kU], rx[kU];
+  uint64_t sum_f[2][2] = {}, sum_s[2][2] = {};  // dgamma of q, k
+  Run run(static_cast<int64_t>(p.T) * p.chunks, p.chunks);
+  uint4 ahead_d[kUb], ahead_x[kUb];
+  auto load = [&](const Run& r) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int h = h0 + u * HPW;
-      rd[u] = rx[u] = make_uint4(0, 0, 0, 0);
-      if (h < p.total_heads)
-        rd[u] = *reinterpret_cast<const uint4*>(p.dy + tok * p.lddy + static_cast<int64_t>(h) * HD + sub * 8);
-      if (p.gq && h < p.heads + p.kv_heads)
-        rx[u] = *reinterpret_cast<const uint4*>(p.x + tok * p.ldx + static_cast<int64_t>(h) * HD + sub * 8);
+    for (int u = 0; u < kUb; ++u) {
+      const int h = r.chunk * (HPW * kUb) + hw + u * HPW;
+      const int64_t col = static_cast<int64_t>(h) * HD;
+      ahead_d[u] = ahead_x[u] = make_uint4(0, 0, 0, 0);
+      if (r.g < r.g1 && h < p.total_heads) ahead_d[u] = at.load(p.dy + r.tok * p.lddy + col);
+      if (r.g < r.g1 && p.gq && h < p.heads + p.kv_heads) ahead_x[u] = at.load(p.x + r.tok * p.ldx + col);
     }
-    int pos = p.rope.pos[tok];
-    if (pos < 0 || pos >= p.rope.n_pos) {
-      if (lane == 0) set_error(p.err, kDevBadIndex);
-      pos = 0;
+  };
+  load(run);
+  Angles ang;
+  int have = -1;
+  while (run.g < run.g1) {
+    const int64_t tok = run.tok;
+    const int run_chunk = run.chunk, h0 = run_chunk * (HPW * kUb) + hw;
+    if (run.tok != have) {
+      const int pos = position(p.rope, run.tok, p.err);
+      if (at.turns) load_angles(ang, p.rope, pos, sub);
+      have = run.tok;
     }
-    Angles ang;
-    load_angles(ang, p.rope, pos, sub);
+    uint4 rd[kUb], rx[kUb];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int h = h0 + u * HPW;
-      const bool is_q = h < p.heads, is_v = h >= p.heads + p.kv_heads;
-      float d[8];
-      unpack8(rd[u], d);
-      rotate<LPH, true>(d, ang, p.rope, sub);
-      if (p.gq) {
-        float x[8], xh[8];
-        unpack8(rx[u], x);
-        float ss = 0.f;
+    for (int u = 0; u < kUb; ++u) {
+      rd[u] = ahead_d[u];
+      rx[u] = ahead_x[u];
+    }
+    run.next(p.chunks);
+    load(run);
+    // Every vector takes the same steps, so that the kUb chains run side by side; v's result
+    // is its input, and vectors past the last are zeros that go nowhere.
+    if (run_chunk * (HPW * kUb) < p.heads + p.kv_heads) {
+      uint64_t df[kUb][2], ds[kUb][2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-        const float r = rsqrtf(head_sum<LPH>(ss) * (1.0f / HD) + p.eps);
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          xh[i] = x[i] * r;
-          const float t = d[i] * xh[i];
-          if (is_q) dgq[i] += t;
-          else if (!is_v) dgk[i] += t;
-          d[i] *= is_q ? gq[i] : gk[i];
-          dot += d[i] * xh[i];
-        }
-        dot = head_sum<LPH>(dot) * (1.0f / HD);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = r * (d[i] - xh[i] * dot);
+      for (int u = 0; u < kUb; ++u) {
+        at.unpack(rd[u], df[u], ds[u]);
+        if (at.turns) rotate<true>(df[u], ds[u], ang);
       }
-      if (h < p.total_heads)
-        *reinterpret_cast<uint4*>(p.dx + tok * p.lddx + static_cast<int64_t>(h) * HD + sub * 8) =
-            is_v ? rd[u] : pack8(d);
+      if (p.gq) {
+        uint64_t xf[kUb][2], xs[kUb][2];
+        float r[kUb], dot[kUb];
+#pragma unroll
+        for (int u = 0; u < kUb; ++u) {
+          at.unpack(rx[u], xf[u], xs[u]);
+          r[u] = dot8(xf[u], xs[u], xf[u], xs[u]);
+        }
+#pragma unroll
+        for (int o = LPH / 2; o; o >>= 1)
+#pragma unroll
+          for (int u = 0; u < kUb; ++u) r[u] += __shfl_xor_sync(0xffffffffu, r[u], o);
+#pragma unroll
+        for (int u = 0; u < kUb; ++u) {
+          const int h = h0 + u * HPW;
+          r[u] = rsqrtf(r[u] * (1.0f / HD) + p.eps);
+          const uint64_t r2 = f2_pack(r[u], r[u]);
+          const bool to_q = h < p.heads, to_k = !to_q && h < p.heads + p.kv_heads;
+          uint64_t gf[2], gs[2];
+          at.gather(gam[h < p.heads ? 0 : 1], gf, gs);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            xf[u][i] = f2_mul(xf[u][i], r2);
+            xs[u][i] = f2_mul(xs[u][i], r2);
+            const uint64_t tf = f2_mul(df[u][i], xf[u][i]), ts = f2_mul(ds[u][i], xs[u][i]);
+            sum_f[0][i] = f2_add(sum_f[0][i], to_q ? tf : 0ull);
+            sum_s[0][i] = f2_add(sum_s[0][i], to_q ? ts : 0ull);
+            sum_f[1][i] = f2_add(sum_f[1][i], to_k ? tf : 0ull);
+            sum_s[1][i] = f2_add(sum_s[1][i], to_k ? ts : 0ull);
+            df[u][i] = f2_mul(df[u][i], gf[i]);
+            ds[u][i] = f2_mul(ds[u][i], gs[i]);
+          }
+          dot[u] = dot8(df[u], ds[u], xf[u], xs[u]);
+        }
+#pragma unroll
+        for (int o = LPH / 2; o; o >>= 1)
+#pragma unroll
+          for (int u = 0; u < kUb; ++u) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], o);
+#pragma unroll
+        for (int u = 0; u < kUb; ++u) {
+          const uint64_t r2 = f2_pack(r[u], r[u]), m2 = f2_pack(dot[u] * (-1.0f / HD), dot[u] * (-1.0f / HD));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            df[u][i] = f2_mul(f2_fma(xf[u][i], m2, df[u][i]), r2);
+            ds[u][i] = f2_mul(f2_fma(xs[u][i], m2, ds[u][i]), r2);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUb; ++u)
+        if (h0 + u * HPW < p.heads + p.kv_heads) rd[u] = at.pack(df[u], ds[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUb; ++u) {
+      const int h = h0 + u * HPW;
+      if (h < p.total_heads) at.store(p.dx + tok * p.lddx + static_cast<int64_t>(h) * HD, rd[u]);
     }
   }
   if (!p.gq) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    red[0][warp * HPW + hw][sub * 8 + i] = dgq[i];
-    red[1][warp * HPW + hw][sub * 8 + i] = dgk[i];
+  for (int w = 0; w < 2; ++w) {
+    float v[8];
+    at.spread(sum_f[w], sum_s[w], v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      red[w][warp * HPW + hw][at.a + i] = v[i];
+      red[w][warp * HPW + hw][at.b + i] = v[4 + i];
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * HD; i += kThreads) {
@@ -410,7 +595,8 @@ __global__ void __launch_bounds__(kThreads) kv_gather_kernel(const GatherParams 
         for (int i = 0; i < 8; ++i)
           v[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? raw[w][u].x : raw[w][u].y) >> (8 * (i & 3)))) *
                  sc[w][u];
-        o = pack8(v);
+        o = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                       pack_bf16x2(v[6], v[7]));
       }
       *reinterpret_cast<uint4*>((w ? p.v_out : p.k_out) + tok * p.ldo + static_cast<int64_t>(h) * HD + sub * 8) = o;
     }
@@ -419,8 +605,8 @@ __global__ void __launch_bounds__(kThreads) kv_gather_kernel(const GatherParams 
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-inline int chunks_of(int total_heads, int hd) {
-  const int per = (32 / (hd / 8)) * kU;
+inline int chunks_of(int total_heads, int hd, int u = kU) {
+  const int per = (32 / (hd / 8)) * u;
   return (total_heads + per - 1) / per;
 }
 inline int log2_exact(int v) {
@@ -445,7 +631,7 @@ bool rope_ok(const QkRopeArgs& a) {
 bool rows_ok(const void* p, int64_t ld, int64_t cols) { return aligned16(p) && ld % 8 == 0 && ld >= cols; }
 
 RopeDev rope_dev(const QkRopeArgs& a) {
-  return {a.rope.cos, a.rope.sin, a.pos, a.rope.n_pos, a.rope.rot, a.rope.half ? 1 : 0};
+  return {a.rope.cos, a.rope.sin, a.pos, a.rope.n_pos, a.rope.rot};
 }
 
 int launch_fwd(const QkRopeArgs& a, int dest, cudaStream_t s) {
@@ -461,11 +647,15 @@ int launch_fwd(const QkRopeArgs& a, int dest, cudaStream_t s) {
   p.n_slots = a.cache.num_pages * a.cache.page_size;
   p.page_shift = dest == kToRows ? 0 : log2_exact(a.cache.page_size);
   p.err = a.err;
-  const int64_t nb = blocks_of(static_cast<int64_t>(a.T) * p.chunks);
-  if (nb < 0) return -1;
+  const int64_t nb = (static_cast<int64_t>(a.T) * p.chunks + kWarps - 1) / kWarps;
   if (nb == 0) return 0;
-  const dim3 grid(static_cast<unsigned>(nb));
-#define RT_FWD(HD, DEST) qk_rope_fwd_kernel<HD, DEST><<<grid, kThreads, 0, s>>>(p)
+  const int most = kCtasPerSm * num_sms();
+  const unsigned grid = static_cast<unsigned>(nb < most ? nb : most);
+#define RT_FWD(HD, DEST)                                                            \
+  do {                                                                              \
+    if (a.rope.half) qk_rope_fwd_kernel<HD, DEST, true><<<grid, kThreads, 0, s>>>(p); \
+    else qk_rope_fwd_kernel<HD, DEST, false><<<grid, kThreads, 0, s>>>(p);          \
+  } while (0)
   if (a.hd == 128) {
     if (dest == kToRows) RT_FWD(128, kToRows);
     else if (dest == kToBf16Pages) RT_FWD(128, kToBf16Pages);
@@ -508,12 +698,13 @@ int kv_append(const QkRopeArgs& in, cudaStream_t s) {
   return launch_fwd(a, a.cache.int8 ? kToInt8Pages : kToBf16Pages, s);
 }
 
-// One CTA holds up to 8 warps of items; 4 CTAs an SM.
+// The backward's grid, a function of the sizes alone (not of the device), fixes the order of
+// the dgamma sums.
 int qk_rope_bwd_blocks(int T, int heads, int kv_heads) {
   if (T <= 0 || heads <= 0 || kv_heads <= 0) return 1;
-  const int64_t groups = static_cast<int64_t>(T) * ((heads + 2 * kv_heads + 2 * kU - 1) / (2 * kU));
+  const int64_t groups = static_cast<int64_t>(T) * ((heads + 2 * static_cast<int64_t>(kv_heads) + 2 * kUb - 1) / (2 * kUb));
   const int64_t b = (groups + kWarps - 1) / kWarps;
-  return static_cast<int>(b < 148 * 4 ? b : 148 * 4);
+  return static_cast<int>(b < 148 * kCtasPerSm ? b : 148 * kCtasPerSm);
 }
 
 int qk_rope_bwd(const QkRopeArgs& a, cudaStream_t s) {
@@ -527,12 +718,17 @@ int qk_rope_bwd(const QkRopeArgs& a, cudaStream_t s) {
   p.gq = a.gamma_q; p.gk = a.gamma_k; p.eps = a.eps;
   p.T = a.T; p.heads = a.heads; p.kv_heads = a.kv_heads;
   p.total_heads = a.heads + a.kv_heads + a.v_heads;
-  p.chunks = chunks_of(p.total_heads, a.hd);
+  p.chunks = chunks_of(p.total_heads, a.hd, kUb);
   p.part = a.partials;
   p.err = a.err;
   const int blocks = qk_rope_bwd_blocks(a.T, a.heads, a.kv_heads);
-  if (a.hd == 128) qk_rope_bwd_kernel<128><<<blocks, kThreads, 0, s>>>(p);
-  else qk_rope_bwd_kernel<64><<<blocks, kThreads, 0, s>>>(p);
+  if (a.hd == 128) {
+    if (a.rope.half) qk_rope_bwd_kernel<128, true><<<blocks, kThreads, 0, s>>>(p);
+    else qk_rope_bwd_kernel<128, false><<<blocks, kThreads, 0, s>>>(p);
+  } else {
+    if (a.rope.half) qk_rope_bwd_kernel<64, true><<<blocks, kThreads, 0, s>>>(p);
+    else qk_rope_bwd_kernel<64, false><<<blocks, kThreads, 0, s>>>(p);
+  }
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !a.gamma_q) return e;
   qk_dgamma_kernel<<<dim3(a.hd / 32, 2), 1024, 0, s>>>(a.partials, blocks, a.dgamma_q, a.dgamma_k, a.hd, a.accumulate);

@@ -109,6 +109,23 @@ def test_qk_norm_rope_forward_and_backward(T, H, Hk, hd, rot, layout, norm):
         assert dgq is None and dgk is None
 
 
+def test_qk_norm_rope_nonfinite_v_stays_in_v():
+    """v passes through; its NaN and Inf, forward and backward, reach nothing of q, k or the gammas."""
+    T, H, Hk, hd = 9, 5, 1, 128
+    g, qkv, pos, rope, gq, gk = rope_case(T, H, Hk, hd, 64, "half", True, seed=2)
+    dout = randn(g, *qkv.shape).bfloat16()
+    exp, exp_d = ops.qk_norm_rope(qkv, pos, rope, H, Hk, gq, gk), ops.qk_norm_rope_backward(dout, qkv, pos, rope, H, Hk, gq, gk)
+    cut = (H + Hk) * hd
+    for t in (qkv, dout):
+        t[3, cut] = float("nan")
+        t[4, cut + 7] = float("inf")
+    out, d = ops.qk_norm_rope(qkv, pos, rope, H, Hk, gq, gk), ops.qk_norm_rope_backward(dout, qkv, pos, rope, H, Hk, gq, gk)
+    assert torch.equal(out[:, :cut], exp[:, :cut]) and torch.equal(d[0][:, :cut], exp_d[0][:, :cut])
+    assert torch.equal(d[1], exp_d[1]) and torch.equal(d[2], exp_d[2])
+    assert torch.equal(out[:, cut:].view(torch.int16), qkv[:, cut:].view(torch.int16))
+    assert torch.equal(d[0][:, cut:].view(torch.int16), dout[:, cut:].view(torch.int16))
+
+
 def test_qk_norm_rope_gradient_against_differences():
     """d(sum w . y)/dx and /dgamma by central differences of the 64-bit forward: a check of the formula
     that shares nothing with autograd."""
