@@ -589,7 +589,7 @@ int attn_paged_few(const paged::Params& p, cudaStream_t s) {
 }
 
 int64_t attn_paged_workspace_bytes(int hd) {
-  const int64_t few = attn_paged_few_ctas() * paged::kBM, many = attn_paged_many_ctas() * 128;
+  const int64_t few = attn_paged_few_ctas() * paged::kBM, many = attn_paged_many_ctas() * 256;
   return paged::kCounterBytes + (few > many ? few : many) * 2 * (hd + 2) * 4;
 }
 
@@ -611,12 +611,12 @@ int attn_paged(const PagedAttnArgs& a, cudaStream_t s) {
   p.max_len = static_cast<int>(room < (1 << 30) ? room : 1 << 30);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   // Up to 16 rows per key head and sequence fill one tile of the kernel above; more rows share
-  // each block's keys in tiles of up to 128 on the tcgen05 tensor cores.
+  // each block's keys in tiles of up to 2 x 128 on the tcgen05 tensor cores.
   if (static_cast<int64_t>(a.max_q) * p.G <= paged::kBM || p.G > 128) {
     p.bm = paged::kBM;
     return attn_paged_few(p, s);
   }
-  p.bm = 128 / p.G * p.G;  // whole tokens, so that a tile of q is one TMA box
+  p.bm = 2 * (128 / p.G * p.G);  // two halves of whole tokens, so that a half of q is one TMA box
   return attn_paged_many(p, s);
 }
 

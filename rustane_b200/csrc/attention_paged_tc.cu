@@ -3,18 +3,23 @@
 // the work and the join as in attention_paged.cu; the products and the softmax are built
 // like the training forward's (attention_tc.cu).
 //
-// Compute-bound on the 4 hd flop per row and visible key; in practice the softmax's issue
-// slots bound it before the tensor pipe.  One persistent CTA per SM:
-//   warp 0      TMA producer: Q of each item (one box: whole tokens x the G heads of the key
-//               head), then the pages of 128-key blocks of K and V, two blocks deep;
-//   warp 1      MMA issuer: S_j = Q K_j^T into one of two TMEM buffers, O += P_j V_j with P as
-//               the TMEM operand; S_{j+1} goes before O += P_j V_j.  It also zeroes the
-//               v rows of a bf16 edge block that no row of the tile sees;
+// Compute-bound on the 4 hd flop per row and visible key; the exponentials (one a score, 16 a
+// clock and SM) take as long as the products at hd 128.  One persistent CTA per SM runs two
+// streams, each with its own S and O in TMEM, its own MMA warp and its own 128 softmax
+// threads, one row each.  A stream takes 64 keys at a time, into two S buffers in turn, so the
+// scores of the next 64 are ready before the weights of the last are in the product.  An item is up to 2 x 128 rows; the streams take a half each and share every K and V
+// tile, or, if the rows fit one half, take the blocks in turn and add up at the end.
+//   warp 0      TMA producer: Q of each item (one box a half: whole tokens x the G heads of the
+//               key head), then the pages of 128-key K and V tiles into one ring;
+//   warps 1, 3  MMA issuers of the two streams: S_{n+1} = Q K^T, then O += P_n V with P (over
+//               S) as the TMEM operand.  They zero the v rows of a bf16 edge tile that no row sees;
 //   warp 2      owns the TMEM allocation;
-//   warps 4-11  softmax, two threads per row (half the keys each), P over S in TMEM, O
-//               rescaled only when the running maximum grew by more than 2^8;
+//   warps 4-11  softmax, 4 warps a stream: the row's maximum, then P; O rescaled only when the
+//               running maximum grew by more than 2^8;
 //   warps 12-15 (int8 cache) turn the codes into bf16 tiles, exactly, one key a thread;
 //               k's scale multiplies the scores and v's the weights, in fp32.
+// (One stream of two threads a row measured 525 TFLOP/s on 4 x 509 tokens over up to 4091; two
+// streams with one S buffer of 128 keys each waited 2300 of 5600 clocks for their next S.)
 // P is rounded to bf16 for the P V product (its sum is not).  All waits are bounded.
 #include "attention_paged.cuh"
 #include "kernels.h"
@@ -23,26 +28,28 @@ namespace rt {
 namespace paged {
 namespace {
 
-constexpr int kBM = 128;
+constexpr int kBM = 128;               // rows of a half
 constexpr int kBK = 128;
 constexpr int kAtomBytes = kBM * 128;  // 64 bf16 columns of 128 rows
 constexpr int kStages8 = 3;            // int8 tiles (k or v) in flight
 constexpr int kScaleSlots = 4;         // blocks whose scales are held
+constexpr int kSub = 64;               // keys that a stream takes at a time
+constexpr int kMaxRing = 8;
 
+// Every wait names a phase by its parity, so a waiter may be at most one phase behind or ahead of
+// its barrier: each role waits for every phase of the barriers that it uses, in order, and both
+// streams hand back every tile, taken or not.
 enum Bar : int {
   kQFull = 0,
-  kQEmpty = 1,   // every S MMA of the item done
-  kKFull = 2,    // [2]
-  kKEmpty = 4,   // [2]
-  kVFull = 6,    // [2]
-  kVEmpty = 8,   // [2]
-  kSFull = 10,   // [2]
-  kSFree = 12,   // [2]
-  kPFull = 14,   // [2] by S buffer: the softmax may finish block g + 1 before P of block g is waited for
-  kPvDone = 16,  // [2]
-  kOFree = 18,   // [2]
-  kDrain = 20,
-  kCodeFull = 21,                           // [kStages8]
+  kQEmpty = 1,                              // both streams' S MMAs of the item done
+  kOFree = 2,                               // both O buffers read
+  kSFull = 3,                               // [2 streams][2 buffers]
+  kPFull = 7,                               // [2 streams][2 buffers]
+  kPvDone = 11,                             // [2 streams][2 buffers]; the buffer is free too
+  kDrain = 15,                              // [2 streams]
+  kTileFull = 17,                           // [kMaxRing] K and V tiles in turn
+  kTileEmpty = kTileFull + kMaxRing,        // [kMaxRing] both streams are done with it
+  kCodeFull = kTileEmpty + kMaxRing,        // [kStages8]
   kCodeEmpty = kCodeFull + kStages8,        // [kStages8]
   kScaleFull = kCodeEmpty + kStages8,       // [kScaleSlots]
   kScaleEmpty = kScaleFull + kScaleSlots,   // [kScaleSlots]
@@ -52,32 +59,81 @@ enum Bar : int {
 template <int HD, bool I8>
 struct Cfg {
   static constexpr int ATOMS = HD / 64;
-  static constexpr int TILE = ATOMS * kAtomBytes;  // Q, K or V in bf16
+  static constexpr int TILE = ATOMS * kAtomBytes;  // a half of Q, K or V in bf16
   static constexpr int ROW8 = HD;                  // bytes of an int8 key
   static constexpr int CODES = kBK * ROW8;
+  static constexpr int RING = HD == 64 ? 8 : I8 ? 3 : 4;
   static constexpr int Q = 0;
-  static constexpr int K = Q + TILE;      // [2]
-  static constexpr int V = K + 2 * TILE;  // [2]
-  static constexpr int CODE = V + 2 * TILE;
-  static constexpr int SCALE = CODE + (I8 ? kStages8 * CODES : 0);              // [slot][k, v][128]
-  static constexpr int RED = SCALE + (I8 ? kScaleSlots * 2 * kBK * 4 : 0);      // float [2][2 halves][128]: row max
-  static constexpr int SUM = RED + 2 * 2 * kBM * 4;                             // float [2 halves][128]
-  static constexpr int NANS = SUM + 2 * kBM * 4;                                // unsigned [4 quadrants][2 halves]
+  static constexpr int KV = Q + 2 * TILE;  // [RING]
+  static constexpr int CODE = KV + RING * TILE;
+  static constexpr int SCALE = CODE + (I8 ? kStages8 * CODES : 0);          // [slot][k, v][128]
+  static constexpr int ML = SCALE + (I8 ? kScaleSlots * 2 * kBK * 4 : 0);   // float [2 streams][128][m, l]
+  static constexpr int NANS = ML + 2 * kBM * 8;                             // unsigned [4 quadrants][2 streams]
   static constexpr int BAR = NANS + 64;
   static constexpr int BYTES = BAR + 512 + 1024;
   static constexpr int THREADS = I8 ? 512 : 384;
 };
 static_assert(kNumBars * 8 + 16 <= 512, "barrier area");
 
+// tmem_ld_wait() that also orders the uses of the loaded registers after it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
 __device__ __forceinline__ void softmax_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-__device__ __forceinline__ void row_pair_bar(int qw) { asm volatile("bar.sync %0, 64;" ::"r"(2 + qw) : "memory"); }
+// the two softmax warps (one a stream) of TMEM lane quadrant qw
+__device__ __forceinline__ void quad_bar(int qw) { asm volatile("bar.sync %0, 64;" ::"r"(2 + qw) : "memory"); }
+
+// Columns col .. col + 3 of row r in a partial result: rows side by side, one a thread.
+__device__ __forceinline__ float4* part_at(float* part, int r, int col) {
+  return reinterpret_cast<float4*>(part) + (col >> 2) * (2 * kBM) + r;
+}
+
+// How an item's part is shared by the two streams.
+struct Share {
+  bool pair;       // halves of the rows (else: blocks in turn)
+  int rows[2];     // rows of each half
+  int lo[2], hi[2];  // keys that each half sees
+  int key0;        // first key of the part
+  __device__ __forceinline__ Share(const Walk<kBK>& w, int half) {
+    const int n = w.rows();
+    pair = n > half;
+    rows[0] = min(n, half);
+    rows[1] = pair ? n - half : rows[0];
+    key0 = (w.blk0 + w.off) * kBK;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      lo[u] = pair ? w.row_lo(u * half) : w.lo;
+      hi[u] = pair ? max(0, w.row_hi(u * half + rows[u] - 1)) : w.hi;
+    }
+  }
+  // whether any row sees the part's block b: others are not loaded (rows of a short window may
+  // leave such blocks between the halves)
+  __device__ __forceinline__ bool loaded(int b) const { return !pair || takes(0, b) || takes(1, b); }
+  // whether stream u works on the part's block b
+  __device__ __forceinline__ bool takes(int u, int b) const {
+    const int k = key0 + b * kBK;
+    return pair ? k < hi[u] && k + kBK > lo[u] : (b & 1) == u;
+  }
+  // whether block b is the last one of stream u in a part of cnt blocks
+  __device__ __forceinline__ bool ends(int u, int b, int cnt) const {
+    return pair ? b + 1 >= cnt || !takes(u, b + 1) : b + 2 >= cnt;
+  }
+  __device__ __forceinline__ int count(int u, int cnt) const {
+    if (!pair) return (cnt + 1 - u) >> 1;
+    const int first = max(0, lo[u] - key0) / kBK, last = min(cnt, (max(0, hi[u] - key0) + kBK - 1) / kBK);
+    return hi[u] > lo[u] && last > first ? last - first : 0;
+  }
+};
 
 template <int HD, bool I8>
 __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
     attn_paged_many_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                            const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Params p, int min_blocks) {
   using C = Cfg<HD, I8>;
-  constexpr int HC = HD / 2;  // output columns per softmax thread
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::BAR);
@@ -85,23 +141,25 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* is_last = abort_flag + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int half = p.bm / 2;
   const PagedAttnArgs& a = p.a;
 
   if (threadIdx.x == 0) {
     mbar_init(&bar[kQFull], 1);
-    mbar_init(&bar[kQEmpty], 1);
+    mbar_init(&bar[kQEmpty], 2);
+    mbar_init(&bar[kOFree], 8);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar[kKFull + i], I8 ? 4 : 1);
-      mbar_init(&bar[kKEmpty + i], 1);
-      mbar_init(&bar[kVFull + i], I8 ? 4 : 1);
-      mbar_init(&bar[kVEmpty + i], 1);
-      mbar_init(&bar[kSFull + i], 1);
-      mbar_init(&bar[kSFree + i], 1);
-      mbar_init(&bar[kPvDone + i], 1);
-      mbar_init(&bar[kOFree + i], 8);
-      mbar_init(&bar[kPFull + i], 8);
+      mbar_init(&bar[kDrain + i], 1);
     }
-    mbar_init(&bar[kDrain], 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bar[kSFull + i], 1);
+      mbar_init(&bar[kPFull + i], 4);
+      mbar_init(&bar[kPvDone + i], 1);
+    }
+    for (int i = 0; i < C::RING; ++i) {
+      mbar_init(&bar[kTileFull + i], I8 ? 4 : 1);
+      mbar_init(&bar[kTileEmpty + i], 2);
+    }
     for (int i = 0; i < kStages8; ++i) {
       mbar_init(&bar[kCodeFull + i], 1);
       mbar_init(&bar[kCodeEmpty + i], 4);
@@ -123,6 +181,9 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
   Walk<kBK> w = start_walk<kBK, C::THREADS>(p, min_blocks, total, P);  // its barriers cover the set-up above
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // columns [0,128) S0, [128,256) S1, then O0, O1 of 128 each
+  auto wait_all = [&](uint64_t* b, uint32_t parity) {  // a whole warp; false: timed out or given up
+    return __all_sync(0xffffffffu, mbar_wait(b, parity) && !*abort_flag);
+  };
 
   if (warp == 0) {
     // ----------------------------------------------------------------- producer
@@ -134,42 +195,46 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
     }
     const int ps = 1 << p.page_shift;
     int g = 0, it = 0;
-    int q_issued = 0, k_issued = 0, v_issued = 0, s_issued = 0;  // k_issued of an int8 cache: k and v tiles
+    int q_issued = 0, t_issued = 0, s_issued = 0;  // t_issued: tiles of the ring, or int8 tiles
     bool ok = true;
-    auto wait = [&](uint64_t* b, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(b, parity) && !*abort_flag);
-    };
     for (; ok && w.more(); w.next()) {
       if (w.empty()) continue;
       const int32_t* table = a.table + w.s * a.table_ld;
       const int cnt = w.count();
       const int key00 = (w.blk0 + w.off) * kBK;
+      const Share sh(w, half);
       auto my_page = [&](int b) {
         const int key = key00 + b * kBK + lane * ps;
         return b < cnt && lane * ps < kBK && key < w.hi && key + ps > w.lo ? page_of(p, table, key) : -1;
       };
-      int page = my_page(0);
-      if (it > 0 && !wait(&bar[kQEmpty], (it - 1) & 1)) {
+      auto after = [&](int b) {
+        do ++b;
+        while (b < cnt && !sh.loaded(b));
+        return b;
+      };
+      int page = my_page(after(-1));
+      if (it > 0 && !wait_all(&bar[kQEmpty], (it - 1) & 1)) {
         ok = false;
         break;
       }
       if (lane == 0) {
-        mbar_arrive_expect_tx(&bar[kQFull], C::ATOMS * p.bm * 128);
+        const int halves = sh.pair ? 2 : 1;
+        mbar_arrive_expect_tx(&bar[kQFull], halves * C::ATOMS * half * 128);
+        for (int u = 0; u < halves; ++u)
 #pragma unroll
-        for (int x = 0; x < C::ATOMS; ++x)
-          tma_load_3d(smem + C::Q + x * kAtomBytes, &tm_q, &bar[kQFull], x * 64, w.h * p.G, w.q0 + w.t * p.bm / p.G);
+          for (int x = 0; x < C::ATOMS; ++x)
+            tma_load_3d(smem + C::Q + u * C::TILE + x * kAtomBytes, &tm_q, &bar[kQFull], x * 64, w.h * p.G,
+                        w.q0 + (w.t * p.bm + u * half) / p.G);
       }
       q_issued = ++it;
-      for (int b = 0; b < cnt; ++b, ++g) {
-        const int ahead = my_page(b + 1);
+      for (int b = after(-1); b < cnt; b = after(b), ++g) {
+        const int ahead = my_page(after(b));
         const int loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
         const int64_t row64 = ((static_cast<int64_t>(page < 0 ? 0 : page) * a.cache.kv_heads + w.h) << p.page_shift);
         const int row = static_cast<int>(row64);
-        const int st = g & 1;
-        const uint32_t ph = (g >> 1) & 1;
         if (I8) {
           const int sl = g % kScaleSlots;
-          if (!wait(&bar[kScaleEmpty + sl], ((g / kScaleSlots) & 1) ^ 1)) {
+          if (!wait_all(&bar[kScaleEmpty + sl], ((g / kScaleSlots) & 1) ^ 1)) {
             ok = false;
             break;
           }
@@ -186,32 +251,25 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const CUtensorMap* tm = kv ? &tm_v : &tm_k;
-          if (I8) {
-            const int x = 2 * g + kv, cs = x % kStages8;
-            if (!wait(&bar[kCodeEmpty + cs], ((x / kStages8) & 1) ^ 1)) {
-              ok = false;
-              break;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(&bar[kCodeFull + cs], loads * ps * C::ROW8);
-            __syncwarp();
-            if (page >= 0)
-              tma_load_2d(smem + C::CODE + cs * C::CODES + lane * ps * C::ROW8, tm, &bar[kCodeFull + cs], 0, row);
-            k_issued = x + 1;
-          } else {
-            const int full = (kv ? kVFull : kKFull) + st, empty = (kv ? kVEmpty : kKEmpty) + st;
-            if (!wait(&bar[empty], ph ^ 1)) {
-              ok = false;
-              break;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(&bar[full], loads * ps * C::ATOMS * 128);
-            __syncwarp();
-            if (page >= 0) {
-              uint8_t* dst = smem + (kv ? C::V : C::K) + st * C::TILE + lane * ps * 128;
-#pragma unroll
-              for (int x = 0; x < C::ATOMS; ++x) tma_load_2d(dst + x * kAtomBytes, tm, &bar[full], x * 128, row);
-            }
-            (kv ? v_issued : k_issued) = g + 1;
+          const int x = 2 * g + kv;
+          const int n = I8 ? kStages8 : C::RING, st = x % n;
+          uint64_t* full = &bar[(I8 ? kCodeFull : kTileFull) + st];
+          if (!wait_all(&bar[(I8 ? kCodeEmpty : kTileEmpty) + st], ((x / n) & 1) ^ 1)) {
+            ok = false;
+            break;
           }
+          if (lane == 0) mbar_arrive_expect_tx(full, loads * ps * (I8 ? C::ROW8 : C::ATOMS * 128));
+          __syncwarp();
+          if (page >= 0) {
+            if (I8) {
+              tma_load_2d(smem + C::CODE + st * C::CODES + lane * ps * C::ROW8, tm, full, 0, row);
+            } else {
+#pragma unroll
+              for (int y = 0; y < C::ATOMS; ++y)
+                tma_load_2d(smem + C::KV + st * C::TILE + y * kAtomBytes + lane * ps * 128, tm, full, y * 128, row);
+            }
+          }
+          t_issued = x + 1;
           __syncwarp();
         }
         if (!ok) break;
@@ -221,101 +279,126 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
     if (!ok) {  // let copies still in flight land before the CTA exits
       if (lane == 0) set_error(a.err, kDevTimeoutProducer);
       *abort_flag = 1;
+      const int n = I8 ? kStages8 : C::RING;
       if (q_issued > 0) mbar_wait(&bar[kQFull], (q_issued - 1) & 1);
-      if (I8) {
-        for (int x = k_issued > kStages8 ? k_issued - kStages8 : 0; x < k_issued; ++x)
-          mbar_wait(&bar[kCodeFull + x % kStages8], (x / kStages8) & 1);
-        for (int x = s_issued > kScaleSlots ? s_issued - kScaleSlots : 0; x < s_issued; ++x)
-          mbar_wait(&bar[kScaleFull + x % kScaleSlots], (x / kScaleSlots) & 1);
-      } else {
-        for (int x = k_issued > 2 ? k_issued - 2 : 0; x < k_issued; ++x) mbar_wait(&bar[kKFull + (x & 1)], (x >> 1) & 1);
-        for (int x = v_issued > 2 ? v_issued - 2 : 0; x < v_issued; ++x) mbar_wait(&bar[kVFull + (x & 1)], (x >> 1) & 1);
-      }
+      for (int x = t_issued > n ? t_issued - n : 0; x < t_issued; ++x)
+        mbar_wait(&bar[(I8 ? kCodeFull : kTileFull) + x % n], (x / n) & 1);
+      for (int x = s_issued > kScaleSlots ? s_issued - kScaleSlots : 0; x < s_issued; ++x)
+        mbar_wait(&bar[kScaleFull + x % kScaleSlots], (x / kScaleSlots) & 1);
     }
-  } else if (warp == 1) {
-    // -------------------------------------------------------------- MMA issuer
-    constexpr uint32_t idesc_s = idesc_bf16_f32(kBM, kBK, false, false);  // Q, K: both hd-contiguous
+  } else if (warp == 1 || warp == 3) {
+    // ------------------------------------------------------- MMA issuer of stream u
+    constexpr uint32_t idesc_s = idesc_bf16_f32(kBM, kSub, false, false);  // Q, K: both hd-contiguous
     constexpr uint32_t idesc_o = idesc_bf16_f32(kBM, HD, false, true);    // P key-contiguous, V hd-contiguous
-    const uint32_t sq = smem_u32(smem + C::Q);
-    auto wait = [&](uint64_t* b, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(b, parity) && !*abort_flag);
-    };
-    auto issue_s = [&](int gg) -> bool {
-      const int st = gg & 1;
-      const uint32_t ph = (gg >> 1) & 1;
-      if (!wait(&bar[kKFull + st], ph) || !wait(&bar[kSFree + st], ph ^ 1)) return false;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t sk = smem_u32(smem + C::K + st * C::TILE);
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kAtomBytes + (kk & 3) * 32;
-          umma_bf16(tmem + st * kBK, smem_desc_sw128(sq + off, 16, 1024), smem_desc_sw128(sk + off, 16, 1024), idesc_s,
-                    kk != 0 ? 1u : 0u);
-        }
-        umma_commit(&bar[kKEmpty + st]);
-        umma_commit(&bar[kSFull + st]);
-      }
-      __syncwarp();
-      return true;
-    };
+    const int u = warp >> 1;
+    const uint32_t ts = tmem + u * 128, to = tmem + 256 + u * 128;
     bool ok = true;
-    int g = 0, it = 0;
+    int g = 0, it = 0, n = 0;  // n: 64-key steps of this stream so far
     for (; ok && w.more(); w.next()) {
       if (w.empty()) continue;
       const int cnt = w.count();
-      const int ob = it & 1;
-      if (!wait(&bar[kQFull], it & 1) || !issue_s(g)) {
+      const Share sh(w, half);
+      const uint32_t sq = smem_u32(smem + C::Q + (sh.pair ? u * C::TILE : 0));
+      if (!wait_all(&bar[kQFull], it & 1)) {
         ok = false;
         break;
       }
-      for (int b = 0; b < cnt; ++b, ++g) {
-        if (b + 1 < cnt) {
-          if (!issue_s(g + 1)) {
-            ok = false;
-            break;
+      // block bb (the CTA's gg-th) -> the next one that the stream takes, or the end; the tiles of
+      // the others are handed back
+      auto forward = [&](int& bb, int& gg) {
+        for (;;) {
+          if (bb >= 0 && sh.loaded(bb)) ++gg;
+          if (++bb >= cnt || sh.takes(u, bb)) return true;
+          if (!sh.loaded(bb)) continue;
+          for (int x = 2 * gg; x < 2 * gg + 2; ++x) {
+            if (!wait_all(&bar[kTileFull + x % C::RING], (x / C::RING) & 1)) return false;
+            if (lane == 0) mbar_arrive(&bar[kTileEmpty + x % C::RING]);
           }
-        } else if (lane == 0) {
-          umma_commit(&bar[kQEmpty]);
-        }
-        const int st = g & 1;
-        if (!wait(&bar[kVFull + st], (g >> 1) & 1)) {
-          ok = false;
-          break;
-        }
-        uint8_t* vt = smem + C::V + st * C::TILE;
-        const int key0 = (w.blk0 + w.off + b) * kBK;
-        if (!I8 && (key0 < w.lo || key0 + kBK > w.hi)) {
-          // keys that no row of the tile sees weigh 0, but what is there may be NaN
-          const int first = max(0, w.lo - key0), last = min(kBK, w.hi - key0);
-#pragma unroll
-          for (int x = 0; x < C::ATOMS; ++x) {
-            uint4* rows = reinterpret_cast<uint4*>(vt + x * kAtomBytes);
-            for (int i = lane; i < first * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
-            for (int i = last * 8 + lane; i < kBK * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
           __syncwarp();
         }
-        if (!wait(&bar[kPFull + st], (g >> 1) & 1) || (b == 0 && it >= 2 && !wait(&bar[kOFree + ob], ((it >> 1) - 1) & 1))) {
-          ok = false;
-          break;
-        }
+      };
+      // S of 64 keys into buffer nn & 1, once P V of step nn - 2 has read its weights there
+      auto issue_s = [&](int bb, int gg, int h, int nn) {
+        const int kx = (2 * gg) % C::RING;
+        if ((h == 0 && !wait_all(&bar[kTileFull + kx], ((2 * gg) / C::RING) & 1)) ||
+            (nn >= 2 && !wait_all(&bar[kPvDone + 2 * u + (nn & 1)], ((nn - 2) >> 1) & 1)))
+          return false;
         tc_fence_after();
         if (lane == 0) {
-          const uint32_t sv = smem_u32(vt);
+          const uint32_t sk = smem_u32(smem + C::KV + kx * C::TILE) + h * (kSub * 128);
 #pragma unroll
-          for (int kk = 0; kk < kBK / 16; ++kk) {
-            const uint32_t acol = st * kBK + (kk < 4 ? kk * 8 : 64 + (kk - 4) * 8);
-            umma_bf16_ts(tmem + (2 + ob) * 128, tmem + acol, smem_desc_sw128(sv + kk * 2048, kAtomBytes, 1024), idesc_o,
-                         (b | kk) != 0 ? 1u : 0u);
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * kAtomBytes + (kk & 3) * 32;
+            umma_bf16(ts + (nn & 1) * kSub, smem_desc_sw128(sq + off, 16, 1024), smem_desc_sw128(sk + off, 16, 1024),
+                      idesc_s, kk != 0 ? 1u : 0u);
           }
-          umma_commit(&bar[kVEmpty + st]);
-          umma_commit(&bar[kPvDone + st]);
-          umma_commit(&bar[kSFree + st]);
+          umma_commit(&bar[kSFull + 2 * u + (nn & 1)]);
+          if (h == 1) umma_commit(&bar[kTileEmpty + kx]);
+          if (h == 1 && sh.ends(u, bb, cnt)) umma_commit(&bar[kQEmpty]);
         }
         __syncwarp();
+        return true;
+      };
+      // With 3 tiles in the ring and blocks in turn, the stream's next K goes where its V is now
+      const bool ahead = C::RING > 3 || sh.pair;
+      int b = -1, gb = g;
+      ok = forward(b, gb);
+      if (ok && b < cnt) {
+        ok = issue_s(b, gb, 0, n);
+      } else if (lane == 0) {
+        mbar_arrive(&bar[kQEmpty]);
       }
+      bool first = true;
+      while (ok && b < cnt) {
+        int b2 = b, g2 = gb;
+        const int vx = (2 * gb + 1) % C::RING;
+        uint8_t* vt = smem + C::KV + vx * C::TILE;
+        for (int h = 0; ok && h < 2; ++h, ++n) {
+          if (h == 0) ok = issue_s(b, gb, 1, n + 1);
+          else if (ahead && !sh.ends(u, b, cnt)) ok = forward(b2, g2) && issue_s(b2, g2, 0, n + 1);
+          if (!ok) break;
+          if (h == 0) {
+            ok = wait_all(&bar[kTileFull + vx], ((2 * gb + 1) / C::RING) & 1);
+            if (!ok) break;
+            const int key0 = sh.key0 + b * kBK;
+            if (!I8 && (key0 < w.lo || key0 + kBK > w.hi)) {
+              // keys that no row of the item sees weigh 0, but what is there may be NaN (both
+              // streams write the same zeros, each before its own product)
+              const int from = max(0, w.lo - key0), to_row = min(kBK, w.hi - key0);
+#pragma unroll
+              for (int x = 0; x < C::ATOMS; ++x) {
+                uint4* rows = reinterpret_cast<uint4*>(vt + x * kAtomBytes);
+                for (int i = lane; i < from * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+                for (int i = to_row * 8 + lane; i < kBK * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
+          }
+          ok = wait_all(&bar[kPFull + 2 * u + (n & 1)], (n >> 1) & 1) &&
+               (!first || it == 0 || wait_all(&bar[kOFree], (it - 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t sv = smem_u32(vt) + h * (kSub * 128);
+#pragma unroll
+            for (int kk = 0; kk < kSub / 16; ++kk)
+              umma_bf16_ts(to, ts + (n & 1) * kSub + kk * 8, smem_desc_sw128(sv + kk * 2048, kAtomBytes, 1024), idesc_o,
+                           first && kk == 0 ? 0u : 1u);
+            umma_commit(&bar[kPvDone + 2 * u + (n & 1)]);
+            if (h == 1) umma_commit(&bar[kTileEmpty + vx]);
+          }
+          __syncwarp();
+          first = false;
+        }
+        if (ok && b2 == b) ok = forward(b2, g2) && (b2 >= cnt || issue_s(b2, g2, 0, n));
+        if (!ok) break;
+        b = b2;
+        gb = g2;
+      }
+      g = gb;  // past the part's last block: every loaded one is counted
+      // a stream without a block in this item still takes part in the O hand-over
+      if (ok && first && it > 0) ok = wait_all(&bar[kOFree], (it - 1) & 1);
       ++it;
     }
     if (!ok) {
@@ -323,8 +406,8 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
       *abort_flag = 1;
     }
     if (lane == 0) {
-      umma_commit(&bar[kDrain]);
-      mbar_wait(&bar[kDrain], 0);
+      umma_commit(&bar[kDrain + u]);
+      mbar_wait(&bar[kDrain + u], 0);
     }
     __syncwarp();
   } else if (I8 && warp >= 12) {
@@ -335,31 +418,32 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
     for (; ok && w.more(); w.next()) {
       if (w.empty()) continue;
       const int cnt = w.count();
-      for (int b = 0; ok && b < 2 * cnt; ++b, ++x) {
-        const int g = x >> 1, st = g & 1, cs = x % kStages8;
-        const bool v = x & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar[kCodeFull + cs], (x / kStages8) & 1) &&
-                                         mbar_wait(&bar[(v ? kVEmpty : kKEmpty) + st], ((g >> 1) & 1) ^ 1) && !*abort_flag);
+      const Share sh(w, half);
+      for (int b = 0; ok && b < 2 * cnt; ++b) {
+        if (!sh.loaded(b >> 1)) continue;
+        const int cs = x % kStages8, st = x % C::RING;
+        ok = wait_all(&bar[kCodeFull + cs], (x / kStages8) & 1) && wait_all(&bar[kTileEmpty + st], ((x / C::RING) & 1) ^ 1);
         if (!ok) break;
         const uint8_t* src = smem + C::CODE + cs * C::CODES + r * C::ROW8;
-        uint8_t* dst = smem + (v ? C::V : C::K) + st * C::TILE + r * 128;
+        uint8_t* dst = smem + C::KV + st * C::TILE + r * 128;
 #pragma unroll
         for (int ch = 0; ch < HD / 16; ++ch) {
           const int sw = HD == 64 ? ch ^ ((r >> 1) & 3) : ch ^ (r & 7);
-          const uint4 u = *reinterpret_cast<const uint4*>(src + sw * 16);
+          const uint4 q = *reinterpret_cast<const uint4*>(src + sw * 16);
           uint8_t* d = dst + (ch >> 2) * kAtomBytes;
           const int c0 = (ch & 3) * 2;
           *reinterpret_cast<uint4*>(d + ((c0 ^ (r & 7)) << 4)) =
-              make_uint4(i8x2_bf16x2<0, 1>(u.x), i8x2_bf16x2<2, 3>(u.x), i8x2_bf16x2<0, 1>(u.y), i8x2_bf16x2<2, 3>(u.y));
+              make_uint4(i8x2_bf16x2<0, 1>(q.x), i8x2_bf16x2<2, 3>(q.x), i8x2_bf16x2<0, 1>(q.y), i8x2_bf16x2<2, 3>(q.y));
           *reinterpret_cast<uint4*>(d + (((c0 + 1) ^ (r & 7)) << 4)) =
-              make_uint4(i8x2_bf16x2<0, 1>(u.z), i8x2_bf16x2<2, 3>(u.z), i8x2_bf16x2<0, 1>(u.w), i8x2_bf16x2<2, 3>(u.w));
+              make_uint4(i8x2_bf16x2<0, 1>(q.z), i8x2_bf16x2<2, 3>(q.z), i8x2_bf16x2<0, 1>(q.w), i8x2_bf16x2<2, 3>(q.w));
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&bar[kCodeEmpty + cs]);
-          mbar_arrive(&bar[(v ? kVFull : kKFull) + st]);
+          mbar_arrive(&bar[kTileFull + st]);
         }
+        ++x;
       }
     }
     if (!ok) {
@@ -367,17 +451,17 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
       *abort_flag = 1;
     }
   } else if (warp >= 4) {
-    // ------------------------------------------------------------------ softmax
-    const int qw = warp & 3;               // TMEM lane quadrant
-    const int hh = (warp - 4) >> 2;        // key columns [64 hh, 64 hh + 64) of the block
-    const int r = qw * 32 + lane;          // row of the tile
+    // ---------------------------------------------------- softmax of stream u, row r
+    const int qw = warp & 3;          // TMEM lane quadrant
+    const int u = (warp - 4) >> 2;
+    const int r = qw * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(qw * 32) << 16;
-    float* red = reinterpret_cast<float*>(smem + C::RED);
-    float* sum = reinterpret_cast<float*>(smem + C::SUM);
+    const uint32_t to = tmem + 256 + lane_off;
+    float* ml = reinterpret_cast<float*>(smem + C::ML);
     volatile unsigned* nans = reinterpret_cast<volatile unsigned*>(smem + C::NANS);
+    const float raise = kRescale / p.scale_log2;
     // A failed (timed-out) wait does not leave the loops: every softmax warp must reach the same
     // sequence of named barriers.  After the first failure every later wait returns at once.
-    const float raise = kRescale / p.scale_log2;
     bool ok = true;
     auto wait = [&](uint64_t* bb, uint32_t parity) {
       bool good = !*abort_flag && mbar_wait(bb, parity);
@@ -387,182 +471,208 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
         *abort_flag = 1;
       }
     };
-    int g = 0, it = 0;
+    int g = 0, n = 0;  // loaded blocks of the CTA, 64-key steps of the stream so far
     for (; w.more(); w.next()) {
-      const int rows = w.rows(), cnt = w.count();
-      const int rr = min(r, rows - 1);
-      const int flat = w.t * p.bm + rr;
-      const int64_t tok = w.q0 + flat / p.G;
-      const int head = w.h * p.G + flat % p.G;
-      __nv_bfloat16* orow = a.out + tok * a.ldo + head * HD + hh * HC;
+      const int cnt = w.count();
+      const Share sh(w, half);
+      const int base = sh.pair ? u * half : 0;  // the stream's first row in the item
+      const bool in = r < sh.rows[u];
+      const int row = base + min(r, sh.rows[u] - 1);
+      const int64_t tok = w.q0 + (w.t * p.bm + row) / p.G;
+      const int head = w.h * p.G + (w.t * p.bm + row) % p.G;
+      __nv_bfloat16* orow = a.out + tok * a.ldo + head * HD;
       float* lse = a.lse2 ? a.lse2 + tok * a.heads + head : nullptr;
       if (w.empty()) {
-        if (r < rows) {
+        if (in && (sh.pair || u == 0)) {
 #pragma unroll
-          for (int i = 0; i < HC / 8; ++i) reinterpret_cast<uint4*>(orow)[i] = make_uint4(0, 0, 0, 0);
-          if (lse && hh == 0) *lse = -CUDART_INF_F;
+          for (int i = 0; i < HD / 8; ++i) reinterpret_cast<uint4*>(orow)[i] = make_uint4(0, 0, 0, 0);
+          if (lse) *lse = -CUDART_INF_F;
         }
         continue;
       }
-      const int ob = it & 1;
-      const uint32_t to = tmem + (2 + ob) * 128 + lane_off + hh * HC;  // this thread's O columns
-      const int hi_r = w.row_hi(rr), lo_r = w.row_lo(rr);
-      const int lo_all = w.row_lo(rows - 1), hi_all = w.row_hi(0);  // keys that every row sees
+      const int hi_r = w.row_hi(row), lo_r = w.row_lo(row);
+      // keys that every row of the stream sees
+      const int lo_all = w.row_lo(base + sh.rows[u] - 1), hi_all = w.row_hi(base);
       float m_used = -CUDART_INF_F, l = 0.f;  // m_used: of the unscaled scores
-      for (int b = 0; b < cnt; ++b, ++g) {
-        const int st = g & 1;
-        const int key0 = (w.blk0 + w.off + b) * kBK;
-        const bool masked = key0 < lo_all || key0 + kBK > hi_all;
-        wait(&bar[kSFull + st], (g >> 1) & 1);
-        tc_fence_after();
-        const uint32_t ts = tmem + st * kBK + lane_off + hh * 64;
-        uint32_t v[64];
-        tmem_ld32(ts, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        tmem_ld32(ts + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-        const float* scales = reinterpret_cast<const float*>(smem + C::SCALE + (g % kScaleSlots) * (2 * kBK * 4)) + hh * 64;
+      bool first = true;
+      for (int b = 0; b < cnt; ++b) {
+        if (!sh.loaded(b)) continue;
         if (I8) wait(&bar[kScaleFull + g % kScaleSlots], (g / kScaleSlots) & 1);
-        tmem_ld_wait();
-        if (I8) {
-#pragma unroll
-          for (int e = 0; e < 64; e += 4) {
-            const float4 k4 = *reinterpret_cast<const float4*>(scales + e);
-            float x0, x1, x2, x3;
-            f2_unpack(f2_mul(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f2_pack(k4.x, k4.y)), x0, x1);
-            f2_unpack(f2_mul(f2_pack(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), f2_pack(k4.z, k4.w)), x2, x3);
-            v[e] = __float_as_uint(x0);
-            v[e + 1] = __float_as_uint(x1);
-            v[e + 2] = __float_as_uint(x2);
-            v[e + 3] = __float_as_uint(x3);
-          }
-        }
-        if (masked) {
-          const int last = hi_r - key0 - hh * 64, first = lo_r - key0 - hh * 64;  // seen: first <= e < last
-#pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (e >= last || e < first) v[e] = __float_as_uint(-CUDART_INF_F);
-        }
-        float mc[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t* u = v + 16 * q;
-          mc[q] = fmax3(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]));
-#pragma unroll
-          for (int e = 3; e < 15; e += 2) mc[q] = fmax3(mc[q], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
-          mc[q] = fmaxf(mc[q], __uint_as_float(u[15]));
-        }
-        float mx = fmax3(mc[0], mc[1], fmaxf(mc[2], mc[3]));
-        red[(st * 2 + hh) * kBM + r] = mx;
-        row_pair_bar(qw);
-        mx = fmaxf(red[(st * 2) * kBM + r], red[(st * 2 + 1) * kBM + r]);
-        const float m_new = fmaxf(m_used, mx);
-        if (b == 0) {
-          m_used = m_new;
-        } else if (__any_sync(0xffffffffu, m_new > m_used + raise)) {
-          wait(&bar[kPvDone + ((g - 1) & 1)], ((g - 1) >> 1) & 1);
-          tc_fence_after();
-          const bool grow = m_new > m_used + raise;
-          const float f = grow ? exp2f((m_used - m_new) * p.scale_log2) : 1.f;
-          if (grow) {
-            l *= f;
-            m_used = m_new;
-          }
 #pragma unroll 1
-          for (int cc = 0; cc < HC / 32; ++cc) {
-            uint32_t o[32];
-            tmem_ld32(to + cc * 32, o);
-            tmem_ld_wait();
+        for (int h = 0; h < 2 && sh.takes(u, b); ++h) {
+          const float* scales = reinterpret_cast<const float*>(smem + C::SCALE + (g % kScaleSlots) * (2 * kBK * 4)) + h * kSub;
+          const int key0 = sh.key0 + b * kBK + h * kSub;
+          const bool masked = key0 < lo_all || key0 + kSub > hi_all;
+          const uint32_t ts = tmem + u * 128 + (n & 1) * kSub + lane_off;
+          wait(&bar[kSFull + 2 * u + (n & 1)], (n >> 1) & 1);
+          tc_fence_after();
+          uint32_t v[2][32];
+          tmem_ld32(ts, v[0]);
+          tmem_ld32(ts + 32, v[1]);
+          tmem_ld_wait(v[0]);
+          tmem_ld_wait(v[1]);
+          if (I8) {  // k's scale
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st32(to + cc * 32, o);
+            for (int e = 0; e < kSub; e += 4) {
+              uint32_t* q = v[e >> 5] + (e & 31);
+              const float4 k4 = *reinterpret_cast<const float4*>(scales + e);
+              float x0, x1, x2, x3;
+              f2_unpack(f2_mul(f2_pack(__uint_as_float(q[0]), __uint_as_float(q[1])), f2_pack(k4.x, k4.y)), x0, x1);
+              f2_unpack(f2_mul(f2_pack(__uint_as_float(q[2]), __uint_as_float(q[3])), f2_pack(k4.z, k4.w)), x2, x3);
+              q[0] = __float_as_uint(x0);
+              q[1] = __float_as_uint(x1);
+              q[2] = __float_as_uint(x2);
+              q[3] = __float_as_uint(x3);
+            }
+          }
+          if (masked) {
+            const int last = hi_r - key0, from = lo_r - key0;  // seen: from <= e < last
+#pragma unroll
+            for (int e = 0; e < kSub; ++e)
+              if (e >= last || e < from) v[e >> 5][e & 31] = __float_as_uint(-CUDART_INF_F);
+          }
+          float mc[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t* x = v[q >> 1] + 16 * (q & 1);
+            mc[q] = fmax3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
+#pragma unroll
+            for (int e = 3; e < 15; e += 2) mc[q] = fmax3(mc[q], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+            mc[q] = fmaxf(mc[q], __uint_as_float(x[15]));
+          }
+          const float m_new = fmaxf(m_used, fmax3(mc[0], mc[1], fmaxf(mc[2], mc[3])));
+          if (first) {
+            m_used = m_new;
+          } else if (__any_sync(0xffffffffu, m_new > m_used + raise)) {
+            wait(&bar[kPvDone + 2 * u + ((n - 1) & 1)], ((n - 1) >> 1) & 1);
+            tc_fence_after();
+            const bool grow = m_new > m_used + raise;
+            const float f = grow ? exp2f((m_used - m_new) * p.scale_log2) : 1.f;
+            if (grow) {
+              l *= f;
+              m_used = m_new;
+            }
+#pragma unroll 1
+            for (int cc = 0; cc < HD / 32; ++cc) {
+              uint32_t o[32];
+              tmem_ld32(to + u * 128 + cc * 32, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(to + u * 128 + cc * 32, o);
+            }
+            tmem_st_wait();
+          }
+          // a maximum of -inf (the row has seen nothing yet) is taken as 0: its weights come out 0.
+          // The difference first: a fused scale * s - m would leave m's rounding, which is
+          // everything where scores are near the lowest value of the type
+          const float ms = m_used == -CUDART_INF_F ? 0.f : m_used;
+          const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), ms2 = f2_pack(ms, ms);
+          uint64_t ls2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+          // P in bf16 pairs over the row's own S columns: keys 2 i, 2 i + 1 at column i
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int tt = 0; tt < 16; ++tt) {
+              const uint32_t s0 = v[c][2 * tt], s1 = v[c][2 * tt + 1];
+              float x0, x1;
+              f2_unpack(f2_mul(f2_sub(f2_pack(__uint_as_float(s0), __uint_as_float(s1)), ms2), sc2), x0, x1);
+              float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+              ls2[c] = f2_add(ls2[c], f2_pack(p0, p1));
+              if (I8) {
+                const float2 vs = *reinterpret_cast<const float2*>(scales + kBK + c * 32 + 2 * tt);
+                f2_unpack(f2_mul(f2_pack(p0, p1), f2_pack(vs.x, vs.y)), p0, p1);
+                if (masked) {  // 0 whatever the scale of an unseen key is
+                  if (s0 == 0xff800000u) p0 = 0.f;
+                  if (s1 == 0xff800000u) p1 = 0.f;
+                }
+              }
+              pk[tt] = pack_bf16x2(p0, p1);
+            }
+            tmem_st16(ts + c * 16, pk);
+          }
+          {
+            float a0, a1, b0, b1;
+            f2_unpack(ls2[0], a0, a1);
+            f2_unpack(ls2[1], b0, b1);
+            l += (a0 + a1) + (b0 + b1);
           }
           tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar[kPFull + 2 * u + (n & 1)]);
+          ++n;
+          first = false;
         }
-        // a maximum of -inf (the row has seen nothing yet) is taken as 0: its weights come out 0
-        const float ms = m_used == -CUDART_INF_F ? 0.f : m_used;
-        // the difference first: a fused scale * s - m would leave m's rounding, which is everything
-        // where scores are near the lowest value of the type
-        const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), ms2 = f2_pack(ms, ms);
-        uint64_t ls2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int tt = 0; tt < 16; ++tt) {
-            const int e = cc * 32 + 2 * tt;
-            float x0, x1;
-            f2_unpack(f2_mul(f2_sub(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), ms2), sc2), x0, x1);
-            float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-            ls2[cc] = f2_add(ls2[cc], f2_pack(p0, p1));
-            if (I8) {
-              const float2 vs = *reinterpret_cast<const float2*>(scales + kBK + e);
-              f2_unpack(f2_mul(f2_pack(p0, p1), f2_pack(vs.x, vs.y)), p0, p1);
-              if (masked) {  // 0 whatever the scale of an unseen key is
-                if (v[e] == 0xff800000u) p0 = 0.f;
-                if (v[e + 1] == 0xff800000u) p1 = 0.f;
-              }
-            }
-            pk[tt] = pack_bf16x2(p0, p1);
-          }
-          tmem_st16(ts + cc * 16, pk);
+        if (I8) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar[kScaleEmpty + g % kScaleSlots]);
         }
-        {
-          float a0, a1, b0, b1;
-          f2_unpack(ls2[0], a0, a1);
-          f2_unpack(ls2[1], b0, b1);
-          l += (a0 + a1) + (b0 + b1);
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bar[kPFull + st]);
-          if (I8) mbar_arrive(&bar[kScaleEmpty + g % kScaleSlots]);
-        }
+        ++g;
       }
       // ------------------------------------------------------------- end of the item (or part)
-      wait(&bar[kPvDone + ((g - 1) & 1)], ((g - 1) >> 1) & 1);
+      // A thread has its row's HD columns (halves), or half of them from both streams' sums.
+      const int c0 = sh.count(0, cnt), c1 = sh.count(1, cnt);
+      if ((u ? c1 : c0) > 0) wait(&bar[kPvDone + 2 * u + ((n - 1) & 1)], ((n - 1) >> 1) & 1);
       tc_fence_after();
-      sum[hh * kBM + r] = l;
-      const bool split = w.off > 0 || cnt < w.nb;
-      const bool may_nan = !I8 && w.n > 1;
-      if (may_nan) {
-        // a row may have met a NaN or an infinity of a key that only a later row sees
-        bool nan = false;
-#pragma unroll 1
-        for (int cc = 0; cc < HC / 32; ++cc) {
-          uint32_t o[32];
-          tmem_ld32(to + cc * 32, o);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) nan = nan || isnan(__uint_as_float(o[e]));
-        }
-        const unsigned word = __ballot_sync(0xffffffffu, nan && r < rows && ok);
-        if (lane == 0) nans[qw * 2 + hh] = word;
+      float f0 = 1.f, f1 = 1.f;  // factors of O0, O1
+      if (sh.pair) {
+        f0 = u == 0 && c0 > 0 ? 1.f : 0.f;
+        f1 = u == 1 && c1 > 0 ? 1.f : 0.f;
+      } else {
+        ml[(u * kBM + r) * 2] = m_used;
+        ml[(u * kBM + r) * 2 + 1] = l;
+        tc_fence_before();
+        quad_bar(qw);  // the other stream's O is complete too
+        tc_fence_after();
+        const float m0 = ml[r * 2], m1 = ml[(kBM + r) * 2];
+        m_used = fmaxf(m0, m1);
+        const float ms = m_used == -CUDART_INF_F ? 0.f : m_used;
+        f0 = exp2f((m0 - ms) * p.scale_log2);
+        f1 = c1 > 0 ? exp2f((m1 - ms) * p.scale_log2) : 0.f;
+        l = ml[r * 2 + 1] * f0 + ml[(kBM + r) * 2 + 1] * f1;
       }
-      row_pair_bar(qw);
-      l = sum[r] + sum[kBM + r];
-      const unsigned todo = may_nan ? nans[qw * 2] | nans[qw * 2 + 1] : 0u;
-      float* part = split ? partial_slot<kBM, HD>(p, blockIdx.x, w.off > 0 ? 0 : 1) : nullptr;
-      const float inv = l == 0.f ? 0.f : 1.f / l, m_log2 = m_used * p.scale_log2;
-      const bool mine = r < rows && !((todo >> lane) & 1u);
-#pragma unroll 1
-      for (int cc = 0; cc < HC / 32; ++cc) {
+      const int col0 = sh.pair ? 0 : u * (HD / 2), chunks = sh.pair ? HD / 32 : HD / 64;
+      // 32 columns of the row's sum; O of a stream without blocks is never read
+      auto column32 = [&](int cc, float (&f)[32]) {
         uint32_t o[32];
-        tmem_ld32(to + cc * 32, o);
-        tmem_ld_wait();
-        if (mine && split) {
-          float4* dst = reinterpret_cast<float4*>(part + r * HD + hh * HC + cc * 32);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = 0.f;
+        if (sh.pair ? u == 0 && c0 > 0 : c0 > 0) {
+          tmem_ld32(to + col0 + cc * 32, o);
+          tmem_ld_wait(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(o[e]) * f0;
+        }
+        if (sh.pair ? u == 1 && c1 > 0 : c1 > 0) {
+          tmem_ld32(to + 128 + col0 + cc * 32, o);
+          tmem_ld_wait(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] = fmaf(__uint_as_float(o[e]), f1, f[e]);
+        }
+      };
+      const bool split = w.off > 0 || cnt < w.nb;
+      float* part = split ? partial_slot<2 * kBM, HD>(p, blockIdx.x, w.off > 0 ? 0 : 1) : nullptr;
+      const float inv = l == 0.f ? 0.f : 1.f / l, m_log2 = m_used * p.scale_log2;
+      bool nan = false;
+#pragma unroll 1
+      for (int cc = 0; cc < chunks; ++cc) {
+        float f[32];
+        column32(cc, f);
+        const int col = col0 + cc * 32;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) nan = nan || isnan(f[e]);
+        if (in && split) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            __stcg(dst + e, make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                        __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3])));
-        } else if (mine && ok) {
-          float f[32];
+            __stcg(part_at(part, row, col + 4 * e), make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]));
+        } else if (in && ok) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] = l == 0.f ? 0.f : __uint_as_float(o[e]) * inv;
+          for (int e = 0; e < 32; ++e) f[e] = l == 0.f ? 0.f : f[e] * inv;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            reinterpret_cast<uint4*>(orow + cc * 32)[e] =
+            reinterpret_cast<uint4*>(orow + col)[e] =
                 make_uint4(pack_bf16x2(f[8 * e], f[8 * e + 1]), pack_bf16x2(f[8 * e + 2], f[8 * e + 3]),
                            pack_bf16x2(f[8 * e + 4], f[8 * e + 5]), pack_bf16x2(f[8 * e + 6], f[8 * e + 7]));
         }
@@ -570,45 +680,56 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar[kOFree + ob]);  // this O buffer can take the item after next
-      if (mine && hh == 0) {
+      if (lane == 0) mbar_arrive(&bar[kOFree]);  // the O buffers can take the next item
+      if (in && (sh.pair || u == 0)) {
         if (split) {
-          __stcg(part + kBM * HD + r, m_log2);
-          __stcg(part + kBM * HD + kBM + r, l);
+          __stcg(part + 2 * kBM * HD + row, m_log2);
+          __stcg(part + 2 * kBM * HD + 2 * kBM + row, l);
         } else if (lse && ok) {
           *lse = l == 0.f ? -CUDART_INF_F : m_log2 + log2f(l);
         }
       }
-      if (todo) {  // the quadrant's two warps share its rows
-        const int seg_lo = (w.blk0 + w.off) * kBK, seg_hi = seg_lo + cnt * kBK;
+      // a row may have met a NaN or an infinity of a key that only a later row sees: it is done
+      // over, alone, and written over
+      unsigned todo = 0;
+      if (!I8 && w.n > 1) {
+        todo = __ballot_sync(0xffffffffu, nan && in && ok);
+        if (!sh.pair) {
+          if (lane == 0) nans[qw * 2 + u] = todo;
+          quad_bar(qw);
+          todo = nans[qw * 2] | nans[qw * 2 + 1];
+        }
+      }
+      if (todo) {
+        const int seg_lo = sh.key0, seg_hi = seg_lo + cnt * kBK;
         int nth = 0;
         for (int x = 0; x < 32; ++x) {
-          if (!((todo >> x) & 1u) || (nth++ & 1) != hh) continue;
-          const int row = qw * 32 + x, fl = w.t * p.bm + row;
+          // of a row that both streams share, the quadrant's two warps take every other one
+          if (!((todo >> x) & 1u) || (!sh.pair && (nth++ & 1) != u)) continue;
+          const int rx = base + qw * 32 + x, fl = w.t * p.bm + rx;
           const int64_t tk = w.q0 + fl / p.G;
           const int hd = w.h * p.G + fl % p.G;
           float rm, rl, ro[HD / 32];
-          row_attend<HD>(p, a.table + w.s * a.table_ld, w.h, a.q + tk * a.ldq + hd * HD, max(w.row_lo(row), seg_lo),
-                         min(w.row_hi(row), seg_hi), rm, rl, ro);
+          row_attend<HD>(p, a.table + w.s * a.table_ld, w.h, a.q + tk * a.ldq + hd * HD, max(w.row_lo(rx), seg_lo),
+                         min(w.row_hi(rx), seg_hi), rm, rl, ro);
           const float rinv = rl == 0.f ? 0.f : 1.f / rl;
 #pragma unroll
           for (int e = 0; e < HD / 32; ++e) {
             const int col = lane * (HD / 32) + e;
-            if (split) __stcg(part + row * HD + col, ro[e]);
+            if (split) __stcg(reinterpret_cast<float*>(part_at(part, rx, col)) + (col & 3), ro[e]);
             else a.out[tk * a.ldo + hd * HD + col] = __float2bfloat16(rl == 0.f ? 0.f : ro[e] * rinv);
           }
           if (lane == 0) {
             if (split) {
-              __stcg(part + kBM * HD + row, rm);
-              __stcg(part + kBM * HD + kBM + row, rl);
+              __stcg(part + 2 * kBM * HD + rx, rm);
+              __stcg(part + 2 * kBM * HD + 2 * kBM + rx, rl);
             } else if (a.lse2) {
               a.lse2[tk * a.heads + hd] = rl == 0.f ? -CUDART_INF_F : rm + log2f(rl);
             }
           }
         }
       }
-      ++it;
-      row_pair_bar(qw);  // sum and nans are read before the next item writes them
+      if (!sh.pair) quad_bar(qw);  // ml and nans are read before the next item writes them
       if (!split) continue;
 
       // ------------------------------------------ the item's CTAs: the last one joins them
@@ -621,41 +742,49 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
       softmax_bar();
       if (*is_last) {
         __threadfence();
-        if (r < rows && ok) {
-          auto slot_of = [&](int cta) { return partial_slot<kBM, HD>(p, cta, cta == cta0 ? 1 : 0); };
+        auto slot_of = [&](int cta) { return partial_slot<2 * kBM, HD>(p, cta, cta == cta0 ? 1 : 0); };
+        // a thread joins 16 or more columns of a row: rows side by side, so that loads coalesce
+        const int rows = w.rows();
+        int wide = 16;
+        while (wide < HD && 256 / (HD / wide) < rows) wide *= 2;
+        const int lanes = 256 / (HD / wide), jr = (threadIdx.x - 128) % lanes, jc = (threadIdx.x - 128) / lanes * wide;
+        if (ok && jr < rows) {
           float jm = -CUDART_INF_F, jl = 0.f;
-          for (int x = cta0; x <= cta1; ++x) jm = fmaxf(jm, __ldcg(slot_of(x) + kBM * HD + r));
-          const float base = jm == -CUDART_INF_F ? 0.f : jm;
+          for (int x = cta0; x <= cta1; ++x) jm = fmaxf(jm, __ldcg(slot_of(x) + 2 * kBM * HD + jr));
+          const float base_m = jm == -CUDART_INF_F ? 0.f : jm;
           for (int x = cta0; x <= cta1; ++x)
-            jl += exp2f(__ldcg(slot_of(x) + kBM * HD + r) - base) * __ldcg(slot_of(x) + kBM * HD + kBM + r);
+            jl += exp2f(__ldcg(slot_of(x) + 2 * kBM * HD + jr) - base_m) * __ldcg(slot_of(x) + 2 * kBM * HD + 2 * kBM + jr);
           const float jinv = jl == 0.f ? 0.f : 1.f / jl;
+          const int fl = w.t * p.bm + jr;
+          const int64_t tk = w.q0 + fl / p.G;
+          const int hd = w.h * p.G + fl % p.G;
 #pragma unroll 1
-          for (int cc = 0; cc < HC / 32; ++cc) {
-            float f[32];
+          for (int col = jc; col < jc + wide; col += 16) {
+            float f[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) f[e] = 0.f;
-            for (int x = cta0; x <= cta1; ++x) {
-              const float* src = slot_of(x);
-              const float wt = exp2f(__ldcg(src + kBM * HD + r) - base);
-              const float4* s4 = reinterpret_cast<const float4*>(src + r * HD + hh * HC + cc * 32);
+            for (int e = 0; e < 16; ++e) f[e] = 0.f;
+#pragma unroll 2
+            for (int x = cta0; x <= cta1; ++x) {  // ascending: a fixed order
+              float* src = slot_of(x);
+              const float wt = exp2f(__ldcg(src + 2 * kBM * HD + jr) - base_m);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float4 u = __ldcg(s4 + e);
-                f[4 * e] += wt * u.x;
-                f[4 * e + 1] += wt * u.y;
-                f[4 * e + 2] += wt * u.z;
-                f[4 * e + 3] += wt * u.w;
+              for (int e = 0; e < 4; ++e) {
+                const float4 q = __ldcg(part_at(src, jr, col + 4 * e));
+                f[4 * e] += wt * q.x;
+                f[4 * e + 1] += wt * q.y;
+                f[4 * e + 2] += wt * q.z;
+                f[4 * e + 3] += wt * q.w;
               }
             }
 #pragma unroll
-            for (int e = 0; e < 32; ++e) f[e] = jl == 0.f ? 0.f : f[e] * jinv;
+            for (int e = 0; e < 16; ++e) f[e] = jl == 0.f ? 0.f : f[e] * jinv;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              reinterpret_cast<uint4*>(orow + cc * 32)[e] =
+            for (int e = 0; e < 2; ++e)
+              reinterpret_cast<uint4*>(a.out + tk * a.ldo + hd * HD + col)[e] =
                   make_uint4(pack_bf16x2(f[8 * e], f[8 * e + 1]), pack_bf16x2(f[8 * e + 2], f[8 * e + 3]),
                              pack_bf16x2(f[8 * e + 4], f[8 * e + 5]), pack_bf16x2(f[8 * e + 6], f[8 * e + 7]));
           }
-          if (lse && hh == 0) *lse = jl == 0.f ? -CUDART_INF_F : jm + log2f(jl);
+          if (a.lse2 && jc == 0) a.lse2[tk * a.heads + hd] = jl == 0.f ? -CUDART_INF_F : jm + log2f(jl);
         }
         if (threadIdx.x == 128) *counter = 0;
       }
@@ -679,7 +808,7 @@ int launch(const Params& p, cudaStream_t s) {
   CUtensorMap tq, tk, tv;
   const uint64_t rows = static_cast<uint64_t>(a.cache.num_pages) * a.cache.kv_heads * a.cache.page_size;
   const uint32_t row_bytes = I8 ? HD : 2 * HD, box = row_bytes < 128 ? row_bytes : 128;
-  if (!make_tmap_heads(&tq, a.q, HD, a.heads, a.T, a.ldq, p.G, p.bm / p.G) ||
+  if (!make_tmap_heads(&tq, a.q, HD, a.heads, a.T, a.ldq, p.G, p.bm / 2 / p.G) ||
       !make_tmap_rows(&tk, a.cache.k, row_bytes, rows, box, a.cache.page_size) ||
       !make_tmap_rows(&tv, a.cache.v, row_bytes, rows, box, a.cache.page_size))
     return -3;
