@@ -614,9 +614,11 @@ int attn_paged(const PagedAttnArgs& a, cudaStream_t s) {
   // each block's keys in tiles of up to 2 x 128 on the tcgen05 tensor cores.
   if (static_cast<int64_t>(a.max_q) * p.G <= paged::kBM || p.G > 128) {
     p.bm = paged::kBM;
+    p.tile_tokens = p.bm % p.G ? 0 : p.bm / p.G;
     return attn_paged_few(p, s);
   }
   p.bm = 2 * (128 / p.G * p.G);  // two halves of whole tokens, so that a half of q is one TMA box
+  p.tile_tokens = p.bm / p.G;
   return attn_paged_many(p, s);
 }
 

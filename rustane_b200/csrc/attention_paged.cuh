@@ -30,6 +30,7 @@ struct Params {
   PagedAttnArgs a;
   int G;           // query heads per key head
   int bm;          // rows per tile
+  int tile_tokens; // bm / G where that is whole, else 0
   int page_shift;
   int max_len;     // tokens a row of the page table holds
   float scale_log2;
@@ -65,19 +66,21 @@ struct Walk {
     tiles = (n * p->G + p->bm - 1) / p->bm;
   }
   __device__ __forceinline__ void tile(int tt) {
-    const int i0 = tt * p->bm / p->G, i1 = min(n - 1, (tt * p->bm + p->bm - 1) / p->G);
+    const int tok = p->tile_tokens;  // a division less
+    const int i0 = tok ? tt * tok : tt * p->bm / p->G;
+    const int i1 = min(n - 1, tok ? i0 + tok - 1 : (tt * p->bm + p->bm - 1) / p->G);
     hi = max(0, len - n + i1 + 1);
     lo = p->a.window > 0 ? max(0, len - n + i0 + 1 - p->a.window) : 0;
     blk0 = lo / BK;
     nb = hi > lo ? (hi + BK - 1) / BK - blk0 : 1;
   }
-  __device__ __forceinline__ int64_t seq_blocks() {
+  __device__ __forceinline__ int64_t head_blocks() {  // of one key head of the sequence
     int64_t b = 0;
     for (int tt = 0; tt < tiles; ++tt) {
       tile(tt);
       b += nb;
     }
-    return b * p->a.cache.kv_heads;
+    return b;
   }
   __device__ __forceinline__ bool more() const { return g < g1; }
   __device__ __forceinline__ bool empty() const { return hi <= lo; }
@@ -114,17 +117,19 @@ struct Walk {
 template <int BK, int NT>
 __device__ __forceinline__ Walk<BK> start_walk(const Params& p, int min_blocks, int64_t& total, int& P) {
   __shared__ int64_t warp_sum[NT / 32];
-  __shared__ int64_t first_rem;
+  __shared__ int64_t first_rem, first_head;  // of the CTA's first block in its sequence; the sequence's blocks a head
   __shared__ int first_seq;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Walk<BK> w;
   w.p = &p;
+  const int heads = p.a.cache.kv_heads;
   const int per = (p.a.nseq + NT - 1) / NT;
   const int s0 = min(tid * per, p.a.nseq), s1 = min(s0 + per, p.a.nseq);
-  int64_t mine = 0;
+  int64_t mine = 0, last = 0;
   for (int s = s0; s < s1; ++s) {
     w.seq(s);
-    mine += w.seq_blocks();
+    last = w.head_blocks();
+    mine += last * heads;
   }
   int64_t incl = mine;
 #pragma unroll
@@ -146,20 +151,28 @@ __device__ __forceinline__ Walk<BK> start_walk(const Params& p, int min_blocks, 
   const int c = blockIdx.x;
   w.g = w.g1 = 0;
   if (c < P) {
-    w.g = total * c / P;
-    w.g1 = total * (c + 1) / P;
+    if (total < (1 << 20)) {  // P <= 1024: 32-bit divisions
+      w.g = static_cast<unsigned>(total) * c / P;
+      w.g1 = static_cast<unsigned>(total) * (c + 1) / P;
+    } else {
+      w.g = total * c / P;
+      w.g1 = total * (c + 1) / P;
+    }
   }
   int64_t at = before + incl - mine;  // blocks before this thread's sequences
   if (c < P && w.g >= at && w.g < at + mine) {
     for (int s = s0; s < s1; ++s) {
-      w.seq(s);
-      const int64_t b = w.seq_blocks();
-      if (w.g < at + b) {
+      if (s1 - s0 > 1) {
+        w.seq(s);
+        last = w.head_blocks();
+      }
+      if (w.g < at + last * heads) {
         first_seq = s;
         first_rem = w.g - at;
+        first_head = last;
         break;
       }
-      at += b;
+      at += last * heads;
     }
   }
   __syncthreads();
@@ -167,9 +180,12 @@ __device__ __forceinline__ Walk<BK> start_walk(const Params& p, int min_blocks, 
   w.s = first_seq;
   w.seq(w.s);
   int64_t rem = first_rem;
-  const int64_t per_head = w.seq_blocks() / p.a.cache.kv_heads;
-  w.h = static_cast<int>(rem / per_head);
-  rem -= w.h * per_head;
+  w.h = 0;
+  if (rem >= first_head) {
+    w.h = first_head < (1 << 30) && rem < (int64_t(1) << 31) ? static_cast<unsigned>(rem) / static_cast<unsigned>(first_head)
+                                                            : static_cast<int>(rem / first_head);
+    rem -= w.h * first_head;
+  }
   for (w.t = 0;; ++w.t) {
     w.tile(w.t);
     if (rem < w.nb) break;
@@ -181,6 +197,7 @@ __device__ __forceinline__ Walk<BK> start_walk(const Params& p, int min_blocks, 
 
 // First and last CTA of the current item: CTA c owns blocks [total c / P, total (c + 1) / P).
 __device__ __forceinline__ int block_owner(int64_t x, int64_t total, int P) {
+  if (total < (1 << 20)) return (static_cast<unsigned>(x + 1) * P - 1) / static_cast<unsigned>(total);
   return static_cast<int>(((x + 1) * P - 1) / total);
 }
 

@@ -16,7 +16,8 @@
 //   warp 2      owns the TMEM allocation;
 //   warps 4-11  softmax, 4 warps a stream: the row's maximum, then P; O rescaled only when the
 //               running maximum grew by more than 2^8;
-//   warps 12-15 (int8 cache) turn the codes into bf16 tiles, exactly, one key a thread;
+//   warps 12, 13 (int8 cache) turn the codes into bf16 tiles, exactly, two keys a thread (four
+//               warps of one key a thread were 9% slower on long chunks: they took issue slots);
 //               k's scale multiplies the scores and v's the weights, in fp32.
 // (One stream of two threads a row measured 525 TFLOP/s on 4 x 509 tokens over up to 4091; two
 // streams with one S buffer of 128 keys each waited 2300 of 5600 clocks for their next S.)
@@ -71,7 +72,7 @@ struct Cfg {
   static constexpr int NANS = ML + 2 * kBM * 8;                             // unsigned [4 quadrants][2 streams]
   static constexpr int BAR = NANS + 64;
   static constexpr int BYTES = BAR + 512 + 1024;
-  static constexpr int THREADS = I8 ? 512 : 384;
+  static constexpr int THREADS = I8 ? 448 : 384;
 };
 static_assert(kNumBars * 8 + 16 <= 512, "barrier area");
 
@@ -122,10 +123,13 @@ struct Share {
   __device__ __forceinline__ bool ends(int u, int b, int cnt) const {
     return pair ? b + 1 >= cnt || !takes(u, b + 1) : b + 2 >= cnt;
   }
+  // stream u's blocks: [first, end), every one (halves) or every other one
+  __device__ __forceinline__ int first(int u) const { return pair ? max(0, lo[u] - key0) / kBK : u; }
+  __device__ __forceinline__ int end(int u, int cnt) const {
+    return !pair ? cnt : hi[u] > lo[u] ? min(cnt, (max(0, hi[u] - key0) + kBK - 1) / kBK) : 0;
+  }
   __device__ __forceinline__ int count(int u, int cnt) const {
-    if (!pair) return (cnt + 1 - u) >> 1;
-    const int first = max(0, lo[u] - key0) / kBK, last = min(cnt, (max(0, hi[u] - key0) + kBK - 1) / kBK);
-    return hi[u] > lo[u] && last > first ? last - first : 0;
+    return pair ? max(0, end(u, cnt) - first(u)) : (cnt + 1 - u) >> 1;
   }
 };
 
@@ -157,12 +161,12 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
       mbar_init(&bar[kPvDone + i], 1);
     }
     for (int i = 0; i < C::RING; ++i) {
-      mbar_init(&bar[kTileFull + i], I8 ? 4 : 1);
+      mbar_init(&bar[kTileFull + i], I8 ? 2 : 1);
       mbar_init(&bar[kTileEmpty + i], 2);
     }
     for (int i = 0; i < kStages8; ++i) {
       mbar_init(&bar[kCodeFull + i], 1);
-      mbar_init(&bar[kCodeEmpty + i], 4);
+      mbar_init(&bar[kCodeEmpty + i], 2);
     }
     for (int i = 0; i < kScaleSlots; ++i) {
       mbar_init(&bar[kScaleFull + i], 1);
@@ -412,7 +416,6 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
     __syncwarp();
   } else if (I8 && warp >= 12) {
     // ------------------------------------------------------------ int8 -> bf16
-    const int r = threadIdx.x - 384;  // key of the block
     int x = 0;
     bool ok = true;
     for (; ok && w.more(); w.next()) {
@@ -424,18 +427,20 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
         const int cs = x % kStages8, st = x % C::RING;
         ok = wait_all(&bar[kCodeFull + cs], (x / kStages8) & 1) && wait_all(&bar[kTileEmpty + st], ((x / C::RING) & 1) ^ 1);
         if (!ok) break;
-        const uint8_t* src = smem + C::CODE + cs * C::CODES + r * C::ROW8;
-        uint8_t* dst = smem + C::KV + st * C::TILE + r * 128;
+        for (int r = threadIdx.x - 384; r < kBK; r += 64) {  // keys of the block
+          const uint8_t* src = smem + C::CODE + cs * C::CODES + r * C::ROW8;
+          uint8_t* dst = smem + C::KV + st * C::TILE + r * 128;
 #pragma unroll
-        for (int ch = 0; ch < HD / 16; ++ch) {
-          const int sw = HD == 64 ? ch ^ ((r >> 1) & 3) : ch ^ (r & 7);
-          const uint4 q = *reinterpret_cast<const uint4*>(src + sw * 16);
-          uint8_t* d = dst + (ch >> 2) * kAtomBytes;
-          const int c0 = (ch & 3) * 2;
-          *reinterpret_cast<uint4*>(d + ((c0 ^ (r & 7)) << 4)) =
-              make_uint4(i8x2_bf16x2<0, 1>(q.x), i8x2_bf16x2<2, 3>(q.x), i8x2_bf16x2<0, 1>(q.y), i8x2_bf16x2<2, 3>(q.y));
-          *reinterpret_cast<uint4*>(d + (((c0 + 1) ^ (r & 7)) << 4)) =
-              make_uint4(i8x2_bf16x2<0, 1>(q.z), i8x2_bf16x2<2, 3>(q.z), i8x2_bf16x2<0, 1>(q.w), i8x2_bf16x2<2, 3>(q.w));
+          for (int ch = 0; ch < HD / 16; ++ch) {
+            const int sw = HD == 64 ? ch ^ ((r >> 1) & 3) : ch ^ (r & 7);
+            const uint4 q = *reinterpret_cast<const uint4*>(src + sw * 16);
+            uint8_t* d = dst + (ch >> 2) * kAtomBytes;
+            const int c0 = (ch & 3) * 2;
+            *reinterpret_cast<uint4*>(d + ((c0 ^ (r & 7)) << 4)) =
+                make_uint4(i8x2_bf16x2<0, 1>(q.x), i8x2_bf16x2<2, 3>(q.x), i8x2_bf16x2<0, 1>(q.y), i8x2_bf16x2<2, 3>(q.y));
+            *reinterpret_cast<uint4*>(d + (((c0 + 1) ^ (r & 7)) << 4)) =
+                make_uint4(i8x2_bf16x2<0, 1>(q.z), i8x2_bf16x2<2, 3>(q.z), i8x2_bf16x2<0, 1>(q.w), i8x2_bf16x2<2, 3>(q.w));
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -495,11 +500,13 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
       const int lo_all = w.row_lo(base + sh.rows[u] - 1), hi_all = w.row_hi(base);
       float m_used = -CUDART_INF_F, l = 0.f;  // m_used: of the unscaled scores
       bool first = true;
-      for (int b = 0; b < cnt; ++b) {
-        if (!sh.loaded(b)) continue;
+      // a bf16 cache: the stream's own blocks; an int8 one: every loaded block's scales pass by
+      const int b_step = I8 || sh.pair ? 1 : 2, b_first = I8 ? 0 : sh.first(u), b_end = I8 ? cnt : sh.end(u, cnt);
+      for (int b = b_first; b < b_end; b += b_step) {
+        if (I8 && !sh.loaded(b)) continue;
         if (I8) wait(&bar[kScaleFull + g % kScaleSlots], (g / kScaleSlots) & 1);
 #pragma unroll 1
-        for (int h = 0; h < 2 && sh.takes(u, b); ++h) {
+        for (int h = I8 && !sh.takes(u, b) ? 2 : 0; h < 2; ++h) {
           const float* scales = reinterpret_cast<const float*>(smem + C::SCALE + (g % kScaleSlots) * (2 * kBK * 4)) + h * kSub;
           const int key0 = sh.key0 + b * kBK + h * kSub;
           const bool masked = key0 < lo_all || key0 + kSub > hi_all;
@@ -507,40 +514,46 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
           wait(&bar[kSFull + 2 * u + (n & 1)], (n >> 1) & 1);
           tc_fence_after();
           uint32_t v[2][32];
+          const int last = hi_r - key0, from = lo_r - key0;  // seen: from <= e < last
+          auto finish = [&](uint32_t (&x)[32], int c) {  // k's scale (int8), -inf where unseen
+            if (I8) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                const float4 k4 = *reinterpret_cast<const float4*>(scales + c * 32 + e);
+                float x0, x1, x2, x3;
+                f2_unpack(f2_mul(f2_pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2_pack(k4.x, k4.y)), x0, x1);
+                f2_unpack(f2_mul(f2_pack(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), f2_pack(k4.z, k4.w)), x2,
+                          x3);
+                x[e] = __float_as_uint(x0);
+                x[e + 1] = __float_as_uint(x1);
+                x[e + 2] = __float_as_uint(x2);
+                x[e + 3] = __float_as_uint(x3);
+              }
+            }
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (c * 32 + e >= last || c * 32 + e < from) x[e] = __float_as_uint(-CUDART_INF_F);
+            }
+          };
+          auto top = [](const uint32_t (&x)[32]) {
+            float mc[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              mc[q] = fmax3(__uint_as_float(x[16 * q]), __uint_as_float(x[16 * q + 1]), __uint_as_float(x[16 * q + 2]));
+#pragma unroll
+              for (int e = 3; e < 15; e += 2)
+                mc[q] = fmax3(mc[q], __uint_as_float(x[16 * q + e]), __uint_as_float(x[16 * q + e + 1]));
+            }
+            return fmaxf(fmaxf(mc[0], __uint_as_float(x[15])), fmaxf(mc[1], __uint_as_float(x[31])));
+          };
           tmem_ld32(ts, v[0]);
           tmem_ld32(ts + 32, v[1]);
           tmem_ld_wait(v[0]);
           tmem_ld_wait(v[1]);
-          if (I8) {  // k's scale
-#pragma unroll
-            for (int e = 0; e < kSub; e += 4) {
-              uint32_t* q = v[e >> 5] + (e & 31);
-              const float4 k4 = *reinterpret_cast<const float4*>(scales + e);
-              float x0, x1, x2, x3;
-              f2_unpack(f2_mul(f2_pack(__uint_as_float(q[0]), __uint_as_float(q[1])), f2_pack(k4.x, k4.y)), x0, x1);
-              f2_unpack(f2_mul(f2_pack(__uint_as_float(q[2]), __uint_as_float(q[3])), f2_pack(k4.z, k4.w)), x2, x3);
-              q[0] = __float_as_uint(x0);
-              q[1] = __float_as_uint(x1);
-              q[2] = __float_as_uint(x2);
-              q[3] = __float_as_uint(x3);
-            }
-          }
-          if (masked) {
-            const int last = hi_r - key0, from = lo_r - key0;  // seen: from <= e < last
-#pragma unroll
-            for (int e = 0; e < kSub; ++e)
-              if (e >= last || e < from) v[e >> 5][e & 31] = __float_as_uint(-CUDART_INF_F);
-          }
-          float mc[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t* x = v[q >> 1] + 16 * (q & 1);
-            mc[q] = fmax3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
-#pragma unroll
-            for (int e = 3; e < 15; e += 2) mc[q] = fmax3(mc[q], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-            mc[q] = fmaxf(mc[q], __uint_as_float(x[15]));
-          }
-          const float m_new = fmaxf(m_used, fmax3(mc[0], mc[1], fmaxf(mc[2], mc[3])));
+          finish(v[0], 0);
+          finish(v[1], 1);
+          const float m_new = fmax3(m_used, top(v[0]), top(v[1]));
           if (first) {
             m_used = m_new;
           } else if (__any_sync(0xffffffffu, m_new > m_used + raise)) {
@@ -572,23 +585,31 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
           // P in bf16 pairs over the row's own S columns: keys 2 i, 2 i + 1 at column i
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
+            const uint32_t(&x)[32] = v[c];
             uint32_t pk[16];
 #pragma unroll
-            for (int tt = 0; tt < 16; ++tt) {
-              const uint32_t s0 = v[c][2 * tt], s1 = v[c][2 * tt + 1];
-              float x0, x1;
-              f2_unpack(f2_mul(f2_sub(f2_pack(__uint_as_float(s0), __uint_as_float(s1)), ms2), sc2), x0, x1);
-              float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-              ls2[c] = f2_add(ls2[c], f2_pack(p0, p1));
+            for (int e = 0; e < 32; e += 4) {
+              float pw[4];
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                float x0, x1;
+                f2_unpack(f2_mul(f2_sub(f2_pack(__uint_as_float(x[e + i]), __uint_as_float(x[e + i + 1])), ms2), sc2), x0, x1);
+                pw[i] = ex2_approx(x0);
+                pw[i + 1] = ex2_approx(x1);
+                ls2[c] = f2_add(ls2[c], f2_pack(pw[i], pw[i + 1]));
+              }
               if (I8) {
-                const float2 vs = *reinterpret_cast<const float2*>(scales + kBK + c * 32 + 2 * tt);
-                f2_unpack(f2_mul(f2_pack(p0, p1), f2_pack(vs.x, vs.y)), p0, p1);
+                const float4 vs = *reinterpret_cast<const float4*>(scales + kBK + c * 32 + e);
+                f2_unpack(f2_mul(f2_pack(pw[0], pw[1]), f2_pack(vs.x, vs.y)), pw[0], pw[1]);
+                f2_unpack(f2_mul(f2_pack(pw[2], pw[3]), f2_pack(vs.z, vs.w)), pw[2], pw[3]);
                 if (masked) {  // 0 whatever the scale of an unseen key is
-                  if (s0 == 0xff800000u) p0 = 0.f;
-                  if (s1 == 0xff800000u) p1 = 0.f;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    if (x[e + i] == 0xff800000u) pw[i] = 0.f;
                 }
               }
-              pk[tt] = pack_bf16x2(p0, p1);
+              pk[e / 2] = pack_bf16x2(pw[0], pw[1]);
+              pk[e / 2 + 1] = pack_bf16x2(pw[2], pw[3]);
             }
             tmem_st16(ts + c * 16, pk);
           }
@@ -763,17 +784,27 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
             float f[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) f[e] = 0.f;
-#pragma unroll 2
-            for (int x = cta0; x <= cta1; ++x) {  // ascending: a fixed order
-              float* src = slot_of(x);
-              const float wt = exp2f(__ldcg(src + 2 * kBM * HD + jr) - base_m);
+            for (int x = cta0; x <= cta1; x += 4) {  // ascending: a fixed order; 4 parts' loads together
+              float wt[4];
+              float4 q[4][4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float4 q = __ldcg(part_at(src, jr, col + 4 * e));
-                f[4 * e] += wt * q.x;
-                f[4 * e + 1] += wt * q.y;
-                f[4 * e + 2] += wt * q.z;
-                f[4 * e + 3] += wt * q.w;
+              for (int i = 0; i < 4; ++i) {
+                float* src = slot_of(min(x + i, cta1));
+                wt[i] = x + i <= cta1 ? __ldcg(src + 2 * kBM * HD + jr) : -CUDART_INF_F;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  q[i][e] = x + i <= cta1 ? __ldcg(part_at(src, jr, col + 4 * e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                wt[i] = exp2f(wt[i] - base_m);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  f[4 * e] += wt[i] * q[i][e].x;
+                  f[4 * e + 1] += wt[i] * q[i][e].y;
+                  f[4 * e + 2] += wt[i] * q[i][e].z;
+                  f[4 * e + 3] += wt[i] * q[i][e].w;
+                }
               }
             }
 #pragma unroll
