@@ -7,16 +7,17 @@
 // A row that sees no key (L < n, or an unused batch slot) gives o = 0, lse2 = -inf.
 //
 // This file: up to 16 rows per key head (a decode step).  HBM-bound: K and V of every
-// visible token are read once, 2 hd bytes a token and head each (int8: hd + 4).  The rows
-// are one m16n8k16 tile, so the matrix instructions do 16 rows' work whatever the number
-// of rows; even so they need a few percent of their rate at the speed HBM delivers.
+// visible token are read once, 2 hd bytes a token and head each (int8: hd + 4).  The keys are
+// the 16 rows of the m16n8k16 products (S^T = K Q^T, O^T = V^T P^T) and the query rows their 8
+// columns, NT times: with the query rows as the 16, a step of 1 to 8 rows issued twice the
+// products and held twice the sums.
 //
-// Two CTAs an SM, 160 threads each: warp 4 streams 64-key blocks by TMA (one box per page
-// and 128 bytes of head, swizzled) into a ring of 96 KB; warps 0-3 take 16 keys of each
-// block for all rows, each with its own running maximum, sum and output, which meet in
+// 160 threads a CTA, three CTAs an SM (NT 2: two): warp 4 streams 64-key blocks by TMA (one box
+// per page and 128 bytes of head, swizzled) into a ring of 64 KB (96 KB); warps 0-3 take 16 keys
+// of each block for all rows, each with its own running maximum, sum and output, which meet in
 // the last block's ring slot when the item (or the CTA's part of it) ends.  P is rounded
 // to bf16 for the P V product (its sum is not): 2^-9 of each weight.  int8 rows become
-// bf16 exactly (|code| <= 127) on their way into the product; k's scale multiplies the
+// bf16 exactly (|code| <= 128) on their way into the product; k's scale multiplies the
 // score, v's the weight, in fp32.
 #include "attention_paged.cuh"
 #include "kernels.h"
@@ -25,28 +26,30 @@ namespace rt {
 namespace paged {
 namespace {
 
-constexpr int kBM = 16;   // rows per tile
 constexpr int kBK = 64;   // keys per block
 constexpr int kConsumers = 4;
 constexpr int kThreads = (kConsumers + 1) * 32;
-constexpr int kRingBytes = 96 * 1024;
 
-template <int HD, bool I8>
+template <int HD, bool I8, int NT>
 struct Cfg {
+  static constexpr int BM = 8 * NT;                    // rows per tile
+  static constexpr int CTAS = NT == 1 ? 3 : 2;         // an SM
+  static constexpr int RING_BYTES = NT == 1 ? 64 * 1024 : 96 * 1024;
   static constexpr int ROW = HD * (I8 ? 1 : 2);  // bytes of a key
   static constexpr int TILE = kBK * ROW;
   static constexpr int SCALES = I8 ? kBK * 4 : 0;
   static constexpr int STAGE = 2 * TILE + 2 * SCALES;  // K, V, scales of k, of v
   static constexpr int SLOT = (STAGE + 1023) / 1024 * 1024;
-  static constexpr int STAGES = kRingBytes / SLOT < 8 ? kRingBytes / SLOT : 8;
+  static constexpr int STAGES = RING_BYTES / SLOT < 8 ? RING_BYTES / SLOT : 8;
   static constexpr int BOX = ROW < 128 ? ROW : 128;  // bytes of a row in one TMA box
   static constexpr int BOXES = ROW / BOX;
   // the four warps' outputs meet CHUNK columns at a time in the last block's slot
-  static constexpr int CHUNK = 2 * TILE / (kConsumers * kBM * 4) < HD ? 2 * TILE / (kConsumers * kBM * 4) : HD;
+  static constexpr int CHUNK = 2 * TILE / (kConsumers * BM * 4) < HD ? 2 * TILE / (kConsumers * BM * 4) : HD;
+  static constexpr int TPR = kConsumers * 32 / BM;  // threads per row at the end
   static constexpr int BAR = STAGES * SLOT;
   static constexpr int ML = BAR + 256;                     // float [warp][row][2]
-  static constexpr int FIX = ML + kConsumers * kBM * 8;    // float [row][2] of recomputed rows
-  static constexpr int BYTES = FIX + kBM * 8 + 64 + 1024;  // + flags, alignment slack
+  static constexpr int FIX = ML + kConsumers * BM * 8;    // float [row][2] of recomputed rows
+  static constexpr int BYTES = FIX + BM * 8 + 64 + 1024;  // + flags, alignment slack
 };
 
 // byte offset of 16-byte chunk ch of row r in a TMA-swizzled tile of kBK rows
@@ -74,13 +77,20 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// 8 x 8 16-bit matrix, a row to 4 lanes: transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-template <int HD, bool I8>
-__global__ void __launch_bounds__(kThreads, 2)
+template <int HD, bool I8, int NT>
+__global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
     attn_paged_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                           const __grid_constant__ Params p, int min_blocks) {
-  using C = Cfg<HD, I8>;
+  using C = Cfg<HD, I8, NT>;
+  constexpr int kBM = C::BM;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR);
@@ -170,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 
   // -------------------------------------------------------------------- consumers
-  constexpr int KS = HD / 16;  // k-steps of Q K^T; groups of 16 output columns of P V
+  constexpr int KS = HD / 16;  // k-steps of K Q^T; groups of 16 output columns of V^T P^T
   const int gr = lane >> 2, c = lane & 3;
   const uint32_t ring = smem_u32(smem);
   int g = 0;
@@ -191,40 +201,53 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int i = (r0 + r) / p.G, hg = w.h * p.G + (r0 + r) % p.G;
       if (a.lse2) a.lse2[static_cast<int64_t>(w.q0 + i) * a.heads + hg] = v;
     };
-    // thread's share of the rows at the end: row er, columns 4 ec + 32 j
-    const int er = threadIdx.x >> 3, ec = threadIdx.x & 7;
+    // thread's share of the rows at the end: row er, columns 4 ec + 4 TPR j
+    const int er = threadIdx.x / C::TPR, ec = threadIdx.x % C::TPR;
     if (w.empty()) {
       if (er < rows) {
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int col = 4 * ec; col < HD; col += 32) write_row4(er, col, zero);
+        for (int col = 4 * ec; col < HD; col += 4 * C::TPR) write_row4(er, col, zero);
         if (ec == 0) write_lse(er, -CUDART_INF_F);
       }
       continue;
     }
 
-    // Q: rows gr and gr + 8.  An int8 key's 16 bytes of a k-step arrive 4 to a thread, so
-    // there the k index 2c, 2c + 1, 2c + 8, 2c + 9 stands for entries 4c .. 4c + 3.
-    uint32_t qa[KS][4];
+    // Q^T: row 8 t + gr.  An int8 key's 16 bytes of a k-step arrive 4 to a thread, so there the
+    // k index 2c, 2c + 1, 2c + 8, 2c + 9 stands for entries 4c .. 4c + 3.
+    uint32_t qb[KS][NT][2];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int r = gr + 8 * hf;
+    for (int t = 0; t < NT; ++t) {
+      const int r = 8 * t + gr;
       const bool in = r < rows;
       const __nv_bfloat16* q = q_ptr(in ? r : 0);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const uint32_t* x = reinterpret_cast<const uint32_t*>(q + ks * 16 + (I8 ? 4 * c : 2 * c));
-        qa[ks][hf] = in ? x[0] : 0u;
-        qa[ks][2 + hf] = in ? x[I8 ? 1 : 4] : 0u;
+        qb[ks][t][0] = in ? x[0] : 0u;
+        qb[ks][t][1] = in ? x[I8 ? 1 : 4] : 0u;
       }
     }
-    float o[2 * KS][4];
+    // O^T of columns dg * 16 ..: entries 0, 1 (rows 8 t + 2c, + 1) of column gr (int8: 2 gr),
+    // entries 2, 3 of column gr + 8 (int8: 2 gr + 1)
+    float o[KS][NT][4];
 #pragma unroll
-    for (int i = 0; i < 2 * KS; ++i)
+    for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
-    const int hi_r[2] = {w.row_hi(min(gr, rows - 1)), w.row_hi(min(gr + 8, rows - 1))};
-    const int lo_r[2] = {w.row_lo(min(gr, rows - 1)), w.row_lo(min(gr + 8, rows - 1))};
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][t][e] = 0.f;
+    float m[NT][2], l[NT][2];
+    int hi_r[NT][2], lo_r[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int r = min(8 * t + 2 * c + x, rows - 1);
+        m[t][x] = -CUDART_INF_F;
+        l[t][x] = 0.f;
+        hi_r[t][x] = w.row_hi(r);
+        lo_r[t][x] = w.row_lo(r);
+      }
     // keys that every row sees
     const int lo_all = w.row_lo(rows - 1), hi_all = w.row_hi(0);
 
@@ -235,20 +258,20 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (!ok) *abort_flag = 1;  // the loops run on without waiting: every warp meets the same barriers
       const uint32_t slot = ring + st * C::SLOT;
       if (ok && key0 < w.hi && key0 + 16 > w.lo) {
-        float s[2][4];
+        float s[NT][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
-        // ------------------------------------------------------------ S = Q K^T
+          for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
+        // ------------------------------------------------- S^T = K Q^T: 16 keys x 8 NT rows
         if (!I8) {
-          const int key = warp * 16 + ((lane >> 4) << 3) + (lane & 7);
+          const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
-            uint32_t kb[4];
-            ldsm4(slot + tile_off<C::ROW>(key, 2 * ks + ((lane >> 3) & 1)), kb);
-            mma16816(s[0], qa[ks], kb[0], kb[1]);
-            mma16816(s[1], qa[ks], kb[2], kb[3]);
+            uint32_t ka[4];
+            ldsm4(slot + tile_off<C::ROW>(key, 2 * ks + (lane >> 4)), ka);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma16816(s[t], ka, qb[ks][t][0], qb[ks][t][1]);
           }
         } else {
           const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
@@ -257,85 +280,93 @@ __global__ void __launch_bounds__(kThreads, 2)
             uint32_t kb[4];
             ldsm4(slot + tile_off<C::ROW>(key, ks + (lane >> 4)), kb);
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              mma16816(s[x & 1], qa[ks + (x >> 1)], i8x2_bf16x2<0, 1>(kb[x]), i8x2_bf16x2<2, 3>(kb[x]));
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t ka[4] = {i8x2_bf16x2<0, 1>(kb[2 * x]), i8x2_bf16x2<0, 1>(kb[2 * x + 1]),
+                                      i8x2_bf16x2<2, 3>(kb[2 * x]), i8x2_bf16x2<2, 3>(kb[2 * x + 1])};
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma16816(s[t], ka, qb[ks + x][t][0], qb[ks + x][t][1]);
+            }
           }
         }
         // ------------------------------------------------- scale, mask, running maximum
-        float vs[2][2];
         const bool masked = key0 < lo_all || key0 + 16 > hi_all;
+        float vs[2] = {1.f, 1.f};
         if (I8) {
-          const float* sc = reinterpret_cast<const float*>(smem + st * C::SLOT + 2 * C::TILE) + warp * 16 + 2 * c;
+          const float* sc = reinterpret_cast<const float*>(smem + st * C::SLOT + 2 * C::TILE) + warp * 16 + gr;
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const float2 ks2 = *reinterpret_cast<const float2*>(sc + 8 * nt);
-            const float2 vs2 = *reinterpret_cast<const float2*>(sc + kBK + 8 * nt);
-            vs[nt][0] = vs2.x;
-            vs[nt][1] = vs2.y;
-            s[nt][0] *= ks2.x;
-            s[nt][1] *= ks2.y;
-            s[nt][2] *= ks2.x;
-            s[nt][3] *= ks2.y;
-          }
+          for (int x = 0; x < 2; ++x) vs[x] = sc[kBK + 8 * x];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] *= sc[8 * (e >> 1)];
         }
-        uint32_t seen = 0xffu;  // bit 4 nt + e
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] *= p.scale_log2;
+          for (int e = 0; e < 4; ++e) s[t][e] *= p.scale_log2;
+        uint32_t seen = 0xffffffffu;  // bit 4 t + e
         if (masked) {
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int key = key0 + 8 * nt + 2 * c + (e & 1);
-              if (key < lo_r[e >> 1] || key >= hi_r[e >> 1]) {
-                s[nt][e] = -CUDART_INF_F;
-                seen &= ~(1u << (4 * nt + e));
+              const int key = key0 + gr + 8 * (e >> 1);
+              if (key < lo_r[t][e & 1] || key >= hi_r[t][e & 1]) {
+                s[t][e] = -CUDART_INF_F;
+                seen &= ~(1u << (4 * t + e));
               }
             }
         }
-        float mx[2];
+        float mx[NT][2];
+        bool grow = false;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          mx[hf] = fmaxf(fmaxf(s[0][2 * hf], s[0][2 * hf + 1]), fmaxf(s[1][2 * hf], s[1][2 * hf + 1]));
-          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
-          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
-        }
-        const bool grow0 = mx[0] > m[0] + kRescale, grow1 = mx[1] > m[1] + kRescale;
-        if (__any_sync(0xffffffffu, grow0 || grow1)) {
-          const float f0 = grow0 ? ex2_approx(m[0] - mx[0]) : 1.f, f1 = grow1 ? ex2_approx(m[1] - mx[1]) : 1.f;
-          if (grow0) m[0] = mx[0];
-          if (grow1) m[1] = mx[1];
-          l[0] *= f0;
-          l[1] *= f1;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 2 * KS; ++i) {
-            o[i][0] *= f0;
-            o[i][1] *= f0;
-            o[i][2] *= f1;
-            o[i][3] *= f1;
+          for (int x = 0; x < 2; ++x) {
+            mx[t][x] = fmaxf(s[t][x], s[t][2 + x]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) mx[t][x] = fmaxf(mx[t][x], __shfl_xor_sync(0xffffffffu, mx[t][x], d));
+            grow = grow || mx[t][x] > m[t][x] + kRescale;
+          }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            float f[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const bool gx = mx[t][x] > m[t][x] + kRescale;
+              f[x] = gx ? ex2_approx(m[t][x] - mx[t][x]) : 1.f;
+              if (gx) m[t][x] = mx[t][x];
+              l[t][x] *= f[x];
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[i][t][e] *= f[e & 1];
           }
         }
-        // a maximum of -inf (nothing seen yet) is taken as 0: the weights come out 0
-        const float ms[2] = {m[0] == -CUDART_INF_F ? 0.f : m[0], m[1] == -CUDART_INF_F ? 0.f : m[1]};
+        // ------------------------------------------------------- P^T: 16 keys x 8 NT rows
+        uint32_t pb[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            s[nt][e] = ex2_approx(s[nt][e] - ms[e >> 1]);
-            l[e >> 1] += s[nt][e];
+            // a maximum of -inf (nothing seen yet) is taken as 0: the weights come out 0
+            const float mm = m[t][e & 1] == -CUDART_INF_F ? 0.f : m[t][e & 1];
+            s[t][e] = ex2_approx(s[t][e] - mm);
+            l[t][e & 1] += s[t][e];
             if (I8) {
-              s[nt][e] *= vs[nt][e & 1];
-              if (masked && !((seen >> (4 * nt + e)) & 1u)) s[nt][e] = 0.f;  // whatever the scale was
+              s[t][e] *= vs[e >> 1];
+              if (masked && !((seen >> (4 * t + e)) & 1u)) s[t][e] = 0.f;  // whatever the scale was
             }
           }
-        const uint32_t pa[4] = {pack_bf16x2(s[0][0], s[0][1]), pack_bf16x2(s[0][2], s[0][3]),
-                                pack_bf16x2(s[1][0], s[1][1]), pack_bf16x2(s[1][2], s[1][3])};
-        // ------------------------------------------------------------- O += P V
+          pb[t][0] = transpose8(pack_bf16x2(s[t][0], s[t][1]));
+          pb[t][1] = transpose8(pack_bf16x2(s[t][2], s[t][3]));
+        }
+        // ----------------------------------------------------------------- O^T += V^T P^T
         const uint32_t vt = slot + C::TILE;
-        const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
         if (!I8) {
+          const int key = warp * 16 + ((lane >> 4) << 3) + (lane & 7);
           // v of keys that no row sees counts as 0, whatever is there
           uint32_t keep[2] = {~0u, ~0u};
           const bool edge = key0 < w.lo || key0 + 16 > w.hi;
@@ -348,27 +379,30 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
 #pragma unroll
           for (int dg = 0; dg < KS; ++dg) {
-            uint32_t vb[4];
-            ldsm4t(vt + tile_off<C::ROW>(key, 2 * dg + (lane >> 4)), vb);
+            uint32_t va[4];
+            ldsm4t(vt + tile_off<C::ROW>(key, 2 * dg + ((lane >> 3) & 1)), va);
             if (edge) {
-              vb[0] &= keep[0];
-              vb[1] &= keep[1];
-              vb[2] &= keep[0];
-              vb[3] &= keep[1];
+              va[0] &= keep[0];
+              va[1] &= keep[0];
+              va[2] &= keep[1];
+              va[3] &= keep[1];
             }
-            mma16816(o[2 * dg], pa, vb[0], vb[1]);
-            mma16816(o[2 * dg + 1], pa, vb[2], vb[3]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma16816(o[dg][t], va, pb[t][0], pb[t][1]);
           }
         } else {
-          // 16 columns give two tiles: their even and their odd entries
+          const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+          // the 16 columns are taken as their even ones, then their odd ones
 #pragma unroll
           for (int dg = 0; dg < KS; dg += 2) {
             uint32_t vb[4];
             ldsm4t(vt + tile_off<C::ROW>(key, dg + (lane >> 4)), vb);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              mma16816(o[2 * (dg + x)], pa, i8x2_bf16x2<0, 2>(vb[2 * x]), i8x2_bf16x2<0, 2>(vb[2 * x + 1]));
-              mma16816(o[2 * (dg + x) + 1], pa, i8x2_bf16x2<1, 3>(vb[2 * x]), i8x2_bf16x2<1, 3>(vb[2 * x + 1]));
+              const uint32_t va[4] = {i8x2_bf16x2<0, 2>(vb[2 * x]), i8x2_bf16x2<1, 3>(vb[2 * x]),
+                                      i8x2_bf16x2<0, 2>(vb[2 * x + 1]), i8x2_bf16x2<1, 3>(vb[2 * x + 1])};
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma16816(o[dg + x][t], va, pb[t][0], pb[t][1]);
             }
           }
         }
@@ -383,14 +417,16 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int last = (g - 1) % C::STAGES;  // still held
     float* buf = reinterpret_cast<float*>(smem + last * C::SLOT);
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
-      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
-      if (c == 0) {
-        ml[(warp * kBM + gr + 8 * hf) * 2] = m[hf];
-        ml[(warp * kBM + gr + 8 * hf) * 2 + 1] = l[hf];
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[t][x] += __shfl_xor_sync(0xffffffffu, l[t][x], d);
+        if (gr == 0) {
+          ml[(warp * kBM + 8 * t + 2 * c + x) * 2] = m[t][x];
+          ml[(warp * kBM + 8 * t + 2 * c + x) * 2 + 1] = l[t][x];
+        }
       }
-    }
     consumer_bar();
     auto merged = [&](int r, float& mm, float& ll) {
       mm = -CUDART_INF_F;
@@ -401,17 +437,19 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int x = 0; x < kConsumers; ++x) ll += ml[(x * kBM + r) * 2 + 1] * ex2_approx(ml[(x * kBM + r) * 2] - base);
     };
-    float f[2], dummy, em, el;
+    float f[NT][2], dummy, em, el;
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      merged(gr + 8 * hf, em, dummy);
-      f[hf] = ex2_approx(m[hf] - (em == -CUDART_INF_F ? 0.f : em));
-    }
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        merged(8 * t + 2 * c + x, em, dummy);
+        f[t][x] = ex2_approx(m[t][x] - (em == -CUDART_INF_F ? 0.f : em));
+      }
     merged(er, em, el);
     const bool split = w.off > 0 || cnt < w.nb;
-    float* part = split ? partial_slot<kBM, HD>(p, blockIdx.x, w.off > 0 ? 0 : 1) : nullptr;
+    float* part = split ? partial_slot<16, HD>(p, blockIdx.x, w.off > 0 ? 0 : 1) : nullptr;
     // columns of a row are swizzled in groups of 8 over the banks
-    auto buf_at = [&](int wp, int r, int col) { return (wp * kBM + r) * C::CHUNK + (col ^ ((r & (C::CHUNK / 8 - 1)) << 3)); };
+    auto buf_at = [&](int wp, int r, int col) { return (wp * kBM + r) * C::CHUNK + (col ^ (((r >> 1) & 3) << 3)); };
     float inv = el == 0.f ? 0.f : 1.f / el;
 #pragma unroll
     for (int ch = 0; ch < HD / C::CHUNK; ++ch) {
@@ -419,27 +457,22 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int dg = ch * C::CHUNK / 16; dg < (ch + 1) * C::CHUNK / 16; ++dg)
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int r = gr + 8 * hf, col = dg * 16 - ch * C::CHUNK;
-          const float x0 = o[2 * dg][2 * hf] * f[hf], x1 = o[2 * dg][2 * hf + 1] * f[hf],
-                      y0 = o[2 * dg + 1][2 * hf] * f[hf], y1 = o[2 * dg + 1][2 * hf + 1] * f[hf];
-          if (I8) {
-            *reinterpret_cast<float4*>(buf + buf_at(warp, r, col + 4 * c)) = make_float4(x0, y0, x1, y1);
-          } else {
-            *reinterpret_cast<float2*>(buf + buf_at(warp, r, col + 2 * c)) = make_float2(x0, x1);
-            *reinterpret_cast<float2*>(buf + buf_at(warp, r, col + 8 + 2 * c)) = make_float2(y0, y1);
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 8 * t + 2 * c + (e & 1), col = dg * 16 - ch * C::CHUNK + (I8 ? 2 * gr + (e >> 1) : gr + 8 * (e >> 1));
+            buf[buf_at(warp, r, col)] = o[dg][t][e] * f[t][e & 1];
           }
-        }
       consumer_bar();
-      float v[C::CHUNK / 32][4];
+      float v[C::CHUNK / (4 * C::TPR)][4];
       bool nan = false;
 #pragma unroll
-      for (int j = 0; j < C::CHUNK / 32; ++j) {
+      for (int j = 0; j < C::CHUNK / (4 * C::TPR); ++j) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[j][e] = 0.f;
 #pragma unroll
         for (int x = 0; x < kConsumers; ++x) {
-          const float4 u = *reinterpret_cast<const float4*>(buf + buf_at(x, er, 4 * ec + 32 * j));
+          const float4 u = *reinterpret_cast<const float4*>(buf + buf_at(x, er, 4 * (ec + C::TPR * j)));
           v[j][0] += u.x;
           v[j][1] += u.y;
           v[j][2] += u.z;
@@ -473,17 +506,17 @@ __global__ void __launch_bounds__(kThreads, 2)
             el = fix[2 * er + 1];
             inv = el == 0.f ? 0.f : 1.f / el;
 #pragma unroll
-            for (int j = 0; j < C::CHUNK / 32; ++j)
+            for (int j = 0; j < C::CHUNK / (4 * C::TPR); ++j)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) v[j][e] = buf[er * HD + 4 * ec + 32 * j + e];
+              for (int e = 0; e < 4; ++e) v[j][e] = buf[er * HD + 4 * (ec + C::TPR * j) + e];
           }
           if (threadIdx.x == 0) *nan_rows = 0;
           consumer_bar();
         }
       }
 #pragma unroll
-      for (int j = 0; j < C::CHUNK / 32; ++j) {
-        const int col = ch * C::CHUNK + 4 * ec + 32 * j;
+      for (int j = 0; j < C::CHUNK / (4 * C::TPR); ++j) {
+        const int col = ch * C::CHUNK + 4 * (ec + C::TPR * j);
         if (split) {
           if (er < rows) __stcg(reinterpret_cast<float4*>(part + er * HD + col), make_float4(v[j][0], v[j][1], v[j][2], v[j][3]));
         } else if (er < rows && ok) {
@@ -498,8 +531,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (lane == 0) mbar_arrive(&empty[last]);
     if (ec == 0) {
       if (split) {
-        __stcg(part + kBM * HD + er, em);
-        __stcg(part + kBM * HD + kBM + er, el);
+        __stcg(part + 16 * HD + er, em);
+        __stcg(part + 16 * HD + 16 + er, el);
       } else if (er < rows && ok) {
         write_lse(er, el == 0.f ? -CUDART_INF_F : em + log2f(el));
       }
@@ -516,22 +549,23 @@ __global__ void __launch_bounds__(kThreads, 2)
     consumer_bar();
     if (!*is_last) continue;
     __threadfence();
-    auto slot_of = [&](int cta) { return partial_slot<kBM, HD>(p, cta, cta == cta0 ? 1 : 0); };
-    float jm = -CUDART_INF_F, jl = 0.f, v[HD / 32][4];
+    auto slot_of = [&](int cta) { return partial_slot<16, HD>(p, cta, cta == cta0 ? 1 : 0); };
+    constexpr int kCols = HD / (4 * C::TPR);
+    float jm = -CUDART_INF_F, jl = 0.f, v[kCols][4];
     const int parts_end = er < rows ? cta1 : cta0 - 1;
-    for (int x = cta0; x <= parts_end; ++x) jm = fmaxf(jm, __ldcg(slot_of(x) + kBM * HD + er));
+    for (int x = cta0; x <= parts_end; ++x) jm = fmaxf(jm, __ldcg(slot_of(x) + 16 * HD + er));
     const float base = jm == -CUDART_INF_F ? 0.f : jm;
 #pragma unroll
-    for (int j = 0; j < HD / 32; ++j)
+    for (int j = 0; j < kCols; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[j][e] = 0.f;
     for (int x = cta0; x <= parts_end; ++x) {
       const float* src = slot_of(x);
-      const float wt = ex2_approx(__ldcg(src + kBM * HD + er) - base);
-      jl += wt * __ldcg(src + kBM * HD + kBM + er);
+      const float wt = ex2_approx(__ldcg(src + 16 * HD + er) - base);
+      jl += wt * __ldcg(src + 16 * HD + 16 + er);
 #pragma unroll
-      for (int j = 0; j < HD / 32; ++j) {
-        const float4 u = __ldcg(reinterpret_cast<const float4*>(src + er * HD + 4 * ec + 32 * j));
+      for (int j = 0; j < kCols; ++j) {
+        const float4 u = __ldcg(reinterpret_cast<const float4*>(src + er * HD + 4 * (ec + C::TPR * j)));
         v[j][0] += wt * u.x;
         v[j][1] += wt * u.y;
         v[j][2] += wt * u.z;
@@ -541,10 +575,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (er < rows && ok) {
       const float jinv = jl == 0.f ? 0.f : 1.f / jl;
 #pragma unroll
-      for (int j = 0; j < HD / 32; ++j) {
+      for (int j = 0; j < kCols; ++j) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[j][e] = jl == 0.f ? 0.f : v[j][e] * jinv;
-        write_row4(er, 4 * ec + 32 * j, v[j]);
+        write_row4(er, 4 * (ec + C::TPR * j), v[j]);
       }
       if (ec == 0) write_lse(er, jl == 0.f ? -CUDART_INF_F : jm + log2f(jl));
     }
@@ -554,42 +588,47 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (!ok && threadIdx.x == 0) set_error(a.err, kDevTimeoutEpilogue);
 }
 
-template <int HD, bool I8>
+int few_ctas(int per_sm) {
+  const int c = per_sm * num_sms();
+  return c < kMaxCtas ? c : kMaxCtas;
+}
+
+template <int HD, bool I8, int NT>
 int launch(const Params& p, cudaStream_t s) {
-  using C = Cfg<HD, I8>;
+  using C = Cfg<HD, I8, NT>;
   CUtensorMap tk, tv;
   const uint64_t rows = static_cast<uint64_t>(p.a.cache.num_pages) * p.a.cache.kv_heads * p.a.cache.page_size;
   const uint32_t box = p.a.cache.page_size < kBK ? p.a.cache.page_size : kBK;
   if (!make_tmap_rows(&tk, p.a.cache.k, C::ROW, rows, C::BOX, box) ||
       !make_tmap_rows(&tv, p.a.cache.v, C::ROW, rows, C::BOX, box))
     return -3;
-  const void* fn = reinterpret_cast<const void*>(attn_paged_few_kernel<HD, I8>);
+  const void* fn = reinterpret_cast<const void*>(attn_paged_few_kernel<HD, I8, NT>);
   const cudaError_t attr = smem_limit_once(fn, C::BYTES);
   if (attr != cudaSuccess) return attr;
   // no more CTAs than the bounds allow blocks (a sequence without keys costs one)
-  const int64_t tiles = (static_cast<int64_t>(p.a.max_q < 1 ? 1 : p.a.max_q) * p.G + kBM - 1) / kBM;
+  const int64_t tiles = (static_cast<int64_t>(p.a.max_q < 1 ? 1 : p.a.max_q) * p.G + C::BM - 1) / C::BM;
   const int64_t keys = p.a.max_kv < 1 ? 1 : p.a.max_kv;
   const int64_t most = p.a.nseq * static_cast<int64_t>(p.a.cache.kv_heads) * tiles * ((keys + kBK - 1) / kBK);
-  const int64_t ctas = attn_paged_few_ctas();
-  attn_paged_few_kernel<HD, I8><<<static_cast<unsigned>(most < ctas ? most : ctas), kThreads, C::BYTES, s>>>(tk, tv, p, 1);
+  const int64_t ctas = few_ctas(C::CTAS);
+  attn_paged_few_kernel<HD, I8, NT><<<static_cast<unsigned>(most < ctas ? most : ctas), kThreads, C::BYTES, s>>>(tk, tv, p, 1);
   return cudaGetLastError();
+}
+
+template <int NT>
+int launch_nt(const Params& p, cudaStream_t s) {
+  if (p.a.cache.hd == 128) return p.a.cache.int8 ? launch<128, true, NT>(p, s) : launch<128, false, NT>(p, s);
+  return p.a.cache.int8 ? launch<64, true, NT>(p, s) : launch<64, false, NT>(p, s);
 }
 
 }  // namespace
 }  // namespace paged
 
-int64_t attn_paged_few_ctas() {
-  const int c = 2 * num_sms();
-  return c < paged::kMaxCtas ? c : paged::kMaxCtas;
-}
-
 int attn_paged_few(const paged::Params& p, cudaStream_t s) {
-  if (p.a.cache.hd == 128) return p.a.cache.int8 ? paged::launch<128, true>(p, s) : paged::launch<128, false>(p, s);
-  return p.a.cache.int8 ? paged::launch<64, true>(p, s) : paged::launch<64, false>(p, s);
+  return p.bm == 8 ? paged::launch_nt<1>(p, s) : paged::launch_nt<2>(p, s);
 }
 
 int64_t attn_paged_workspace_bytes(int hd) {
-  const int64_t few = attn_paged_few_ctas() * paged::kBM, many = attn_paged_many_ctas() * 256;
+  const int64_t few = int64_t(paged::kMaxCtas) * 16, many = attn_paged_many_ctas() * 256;
   return paged::kCounterBytes + (few > many ? few : many) * 2 * (hd + 2) * 4;
 }
 
@@ -610,10 +649,10 @@ int attn_paged(const PagedAttnArgs& a, cudaStream_t s) {
   const int64_t room = a.table_ld * a.cache.page_size;
   p.max_len = static_cast<int>(room < (1 << 30) ? room : 1 << 30);
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  // Up to 16 rows per key head and sequence fill one tile of the kernel above; more rows share
+  // Up to 8 or 16 rows per key head and sequence fill one tile of the kernel above; more rows share
   // each block's keys in tiles of up to 2 x 128 on the tcgen05 tensor cores.
-  if (static_cast<int64_t>(a.max_q) * p.G <= paged::kBM || p.G > 128) {
-    p.bm = paged::kBM;
+  if (static_cast<int64_t>(a.max_q) * p.G <= 16 || p.G > 128) {
+    p.bm = static_cast<int64_t>(a.max_q) * p.G <= 8 ? 8 : 16;
     p.tile_tokens = p.bm % p.G ? 0 : p.bm / p.G;
     return attn_paged_few(p, s);
   }

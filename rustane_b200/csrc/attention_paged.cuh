@@ -252,7 +252,6 @@ __device__ __noinline__ void row_attend(const Params& p, const int32_t* table, i
 }  // namespace paged
 
 int attn_paged_few(const paged::Params& p, cudaStream_t s);
-int64_t attn_paged_few_ctas();
 int attn_paged_many(const paged::Params& p, cudaStream_t s);
 int64_t attn_paged_many_ctas();
 
