@@ -514,8 +514,8 @@ typedef struct rt_logit_rules {
 /* out [B, ldo] (may be logits) fp32: tokens that occur in hist divide a positive logit by
  * repetition[b] and multiply another; those in the answer lose frequency * count + presence;
  * then biases; then -inf where the mask forbids.  token (nullable): the first index of the
- * row's largest value, -1 if nothing is above -inf (NaN is never chosen).  An id outside
- * [0, V) is skipped and sets dev_err. */
+ * row's largest value, -1 if nothing is above -inf (NaN is never chosen).  An id of -1 is a
+ * place not yet written and counts for nothing; another one outside [0, V) sets dev_err. */
 RT_API int rt_kernel_logits_adjust(const float* logits, int64_t ldl, float* out, int64_t ldo, int32_t* token, int B,
                                    int V, const rt_logit_rules* rules, int* dev_err, void* stream);
 

@@ -121,8 +121,8 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const Params
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
           const int64_t j = j0 + u * kThreads;
-          if (j < h1 && (id[u] < 0 || id[u] >= a.V)) set_error(a.err, kDevBadToken);
-          else if (id[u] >= id_lo && id[u] < id_hi && j < h1) {
+          if (j < h1 && (id[u] < -1 || id[u] >= a.V)) set_error(a.err, kDevBadToken);
+          else if (id[u] >= max(id_lo, 0) && id[u] < id_hi && j < h1) {
             if (j < made0) atomicOr(&cnt[id[u] - id_lo], kSeen);
             else atomicAdd(&cnt[id[u] - id_lo], 1u);
           }
@@ -130,8 +130,8 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const Params
       }
       for (int64_t j = b0 + tid; j < b1; j += kThreads) {
         const int id = a.bias_ids[j];
-        if (id < 0 || id >= a.V) set_error(a.err, kDevBadToken);
-        else if (id >= id_lo && id < id_hi) atomicOr(&cnt[id - id_lo], kBiased);
+        if (id < -1 || id >= a.V) set_error(a.err, kDevBadToken);
+        else if (id >= max(id_lo, 0) && id < id_hi) atomicOr(&cnt[id - id_lo], kBiased);
       }
       __syncthreads();
     }
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const Params
           if (j < b1) {
             id = a.bias_ids[j];
             val = a.bias_vals[j];
-            if (id < id_lo || id >= id_hi) id = -1;
+            if (id < max(id_lo, 0) || id >= id_hi) id = -1;
           }
           const uint32_t same = __match_any_sync(0xffffffffu, id);
           const bool leader = id >= 0 && (same & ((1u << tid) - 1)) == 0;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const Params
       __syncthreads();
       for (int64_t j = b0 + tid; j < b1; j += kThreads) {  // entries of one token write the same value
         const int id = a.bias_ids[j];
-        if (id < id_lo || id >= id_hi) continue;
+        if (id < max(id_lo, 0) || id >= id_hi) continue;
         float l = __uint_as_float(cnt[id - id_lo]);
         if (!allowed(id)) l = -INFINITY;
         consider(l, id);
