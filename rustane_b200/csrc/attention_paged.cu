@@ -16,9 +16,16 @@
 // per page and 128 bytes of head, swizzled) into a ring of 64 KB (96 KB); warps 0-3 take 16 keys
 // of each block for all rows, each with its own running maximum, sum and output, which meet in
 // the last block's ring slot when the item (or the CTA's part of it) ends.  P is rounded
-// to bf16 for the P V product (its sum is not): 2^-9 of each weight.  int8 rows become
-// bf16 exactly (|code| <= 128) on their way into the product; k's scale multiplies the
-// score, v's the weight, in fp32.
+// to bf16 for the P V product (its sum is not): 2^-9 of each weight.
+//
+// int8: the codes become fp16, exactly (two and a half instructions a pair, one and a half of
+// them on the integer pipe; bf16 takes four and three, and that pipe was the limit: 354 us
+// for 48 x up to 6011 tokens of 32 heads).  q is brought into fp16's range by one power of two
+// per item, exact down to 2^-22 of the largest entry; k's scale multiplies the score in fp32.
+// The weights times v's scales are rounded to fp16 (2^-11 of each) in units of 2^kv, a power of
+// two that a warp moves, with its sums, when its largest weight leaves [2^0, 2^15) units.
+#include <cuda_fp16.h>
+
 #include "attention_paged.cuh"
 #include "kernels.h"
 
@@ -77,6 +84,26 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16816h(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Codes I and J of a word whose sign bits are flipped (codes + 128), in fp16: 1024 + (code + 128)
+// is exact with the codes as the last mantissa bits, and so is the difference.
+template <int I, int J>
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t flipped) {
+  const uint32_t x = __byte_perm(flipped, 0x64646464u, I | 0x40 | (J << 8) | 0x4000), y = 0x64806480u;  // 1152
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float power_of_2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 // 8 x 8 16-bit matrix, a row to 4 lanes: transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -227,6 +254,31 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
         qb[ks][t][1] = in ? x[I8 ? 1 : 4] : 0u;
       }
     }
+    float s_scale = p.scale_log2;
+    int kv = 0;  // int8: O is in units of 2^kv
+    if (I8) {
+      // the largest finite entry to [2^8, 2^9)
+      unsigned top = 0;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const unsigned hi16 = qb[ks][t][x] >> 16 & 0x7fffu, lo16 = qb[ks][t][x] & 0x7fffu;
+            top = max(top, max(hi16 < 0x7f80u ? hi16 : 0u, lo16 < 0x7f80u ? lo16 : 0u));
+          }
+      top = __reduce_max_sync(0xffffffffu, top);
+      const int eq = max(-100, static_cast<int>(top >> 7) - 127 - 8);
+      const float down = power_of_2(-eq);
+      s_scale *= power_of_2(eq);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) qb[ks][t][x] = pack_f16x2(bf16lo(qb[ks][t][x]) * down, bf16hi(qb[ks][t][x]) * down);
+    }
     // O^T of columns dg * 16 ..: entries 0, 1 (rows 8 t + 2c, + 1) of column gr (int8: 2 gr),
     // entries 2, 3 of column gr + 8 (int8: 2 gr + 1)
     float o[KS][NT][4];
@@ -281,29 +333,29 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
             ldsm4(slot + tile_off<C::ROW>(key, ks + (lane >> 4)), kb);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const uint32_t ka[4] = {i8x2_bf16x2<0, 1>(kb[2 * x]), i8x2_bf16x2<0, 1>(kb[2 * x + 1]),
-                                      i8x2_bf16x2<2, 3>(kb[2 * x]), i8x2_bf16x2<2, 3>(kb[2 * x + 1])};
+              const uint32_t k0 = kb[2 * x] ^ 0x80808080u, k1 = kb[2 * x + 1] ^ 0x80808080u;
+              const uint32_t ka[4] = {codes_f16x2<0, 1>(k0), codes_f16x2<0, 1>(k1), codes_f16x2<2, 3>(k0),
+                                      codes_f16x2<2, 3>(k1)};
 #pragma unroll
-              for (int t = 0; t < NT; ++t) mma16816(s[t], ka, qb[ks + x][t][0], qb[ks + x][t][1]);
+              for (int t = 0; t < NT; ++t) mma16816h(s[t], ka, qb[ks + x][t][0], qb[ks + x][t][1]);
             }
           }
         }
         // ------------------------------------------------- scale, mask, running maximum
         const bool masked = key0 < lo_all || key0 + 16 > hi_all;
-        float vs[2] = {1.f, 1.f};
+        float vs[2] = {1.f, 1.f}, ss[2] = {s_scale, s_scale};
         if (I8) {
           const float* sc = reinterpret_cast<const float*>(smem + st * C::SLOT + 2 * C::TILE) + warp * 16 + gr;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) vs[x] = sc[kBK + 8 * x];
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][e] *= sc[8 * (e >> 1)];
+          for (int x = 0; x < 2; ++x) {
+            ss[x] *= sc[8 * x];
+            vs[x] = sc[kBK + 8 * x];
+          }
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[t][e] *= p.scale_log2;
+          for (int e = 0; e < 4; ++e) s[t][e] *= ss[e >> 1];
         uint32_t seen = 0xffffffffu;  // bit 4 t + e
         if (masked) {
 #pragma unroll
@@ -328,7 +380,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
             for (int d = 4; d < 32; d <<= 1) mx[t][x] = fmaxf(mx[t][x], __shfl_xor_sync(0xffffffffu, mx[t][x], d));
             grow = grow || mx[t][x] > m[t][x] + kRescale;
           }
-        if (__any_sync(0xffffffffu, grow)) {
+        const bool raised = __any_sync(0xffffffffu, grow);
+        if (raised) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             float f[2];
@@ -360,8 +413,40 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
               if (masked && !((seen >> (4 * t + e)) & 1u)) s[t][e] = 0.f;  // whatever the scale was
             }
           }
-          pb[t][0] = transpose8(pack_bf16x2(s[t][0], s[t][1]));
-          pb[t][1] = transpose8(pack_bf16x2(s[t][2], s[t][3]));
+          if (!I8) {
+            pb[t][0] = transpose8(pack_bf16x2(s[t][0], s[t][1]));
+            pb[t][1] = transpose8(pack_bf16x2(s[t][2], s[t][3]));
+          }
+        }
+        if (I8) {
+          unsigned top = 0;  // the largest finite weight
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const unsigned x = __float_as_uint(s[t][e]) & 0x7fffffffu;
+              top = max(top, x < 0x7f800000u ? x : 0u);
+            }
+          top = __reduce_max_sync(0xffffffffu, top);
+          const int above = static_cast<int>(top >> 23) - 127 - kv;
+          // too large for fp16, or, where the weights' own unit has just moved, small
+          if (top && (above >= 15 || (raised && above < 0))) {
+            const int to = max(max(-100, kv - 120), min(120, kv + above - 10));
+            const float f = ldexpf(1.f, kv - to);
+            kv = to;
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][t][e] *= f;
+          }
+          const float unit = power_of_2(-kv);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            pb[t][0] = transpose8(pack_f16x2(s[t][0] * unit, s[t][1] * unit));
+            pb[t][1] = transpose8(pack_f16x2(s[t][2] * unit, s[t][3] * unit));
+          }
         }
         // ----------------------------------------------------------------- O^T += V^T P^T
         const uint32_t vt = slot + C::TILE;
@@ -399,10 +484,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
             ldsm4t(vt + tile_off<C::ROW>(key, dg + (lane >> 4)), vb);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const uint32_t va[4] = {i8x2_bf16x2<0, 2>(vb[2 * x]), i8x2_bf16x2<1, 3>(vb[2 * x]),
-                                      i8x2_bf16x2<0, 2>(vb[2 * x + 1]), i8x2_bf16x2<1, 3>(vb[2 * x + 1])};
+              const uint32_t v0 = vb[2 * x] ^ 0x80808080u, v1 = vb[2 * x + 1] ^ 0x80808080u;
+              const uint32_t va[4] = {codes_f16x2<0, 2>(v0), codes_f16x2<1, 3>(v0), codes_f16x2<0, 2>(v1),
+                                      codes_f16x2<1, 3>(v1)};
 #pragma unroll
-              for (int t = 0; t < NT; ++t) mma16816(o[dg + x][t], va, pb[t][0], pb[t][1]);
+              for (int t = 0; t < NT; ++t) mma16816h(o[dg + x][t], va, pb[t][0], pb[t][1]);
             }
           }
         }
@@ -444,6 +530,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
       for (int x = 0; x < 2; ++x) {
         merged(8 * t + 2 * c + x, em, dummy);
         f[t][x] = ex2_approx(m[t][x] - (em == -CUDART_INF_F ? 0.f : em));
+        if (I8) f[t][x] *= power_of_2(kv);
       }
     merged(er, em, el);
     const bool split = w.off > 0 || cnt < w.nb;

@@ -28,6 +28,11 @@ from . import _lib
 from ._lib import RtKvPages, RtLogitRules, RtRope, RustaneError, lib
 
 
+_DENSE = torch.contiguous_format
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+
+
 def _fail(msg: str):
     raise ValueError(msg)
 
@@ -35,17 +40,17 @@ def _fail(msg: str):
 def _rows(name: str, t: torch.Tensor, cols: int, dtype: torch.dtype, device: torch.device, rows: int | None = None) -> int:
     """Checks a row matrix; its row stride, which torch leaves arbitrary where there are fewer than two rows."""
     shape = t.shape
-    if len(shape) != 2 or t.dtype != dtype or shape[1] != cols or (rows is not None and shape[0] != rows):
+    if t.dtype is not dtype or len(shape) != 2 or shape[1] != cols or (rows is not None and shape[0] != rows):
         _fail(f"{name}: expected a [{'T' if rows is None else rows}, {cols}] {dtype} tensor, got {tuple(shape)} {t.dtype}")
     ld, step = t.stride()
-    if t.device != device or (shape[0] and step != 1):
+    if (step != 1 and shape[0]) or t.device != device:
         _fail(f"{name}: its rows have to be contiguous and on {device}")
     return ld if shape[0] > 1 else max(ld, cols)
 
 
 def _vec(name: str, t: torch.Tensor, n: int | None, dtype: torch.dtype, device: torch.device) -> None:
     shape = t.shape
-    if t.dtype != dtype or len(shape) != 1 or (n is not None and shape[0] != n):
+    if t.dtype is not dtype or len(shape) != 1 or (n is not None and shape[0] != n):
         _fail(f"{name}: expected {'a vector' if n is None else n} of {dtype}, got {tuple(shape)} {t.dtype}")
     if t.device != device or not t.is_contiguous():
         _fail(f"{name}: has to be contiguous and on {device}")
@@ -63,14 +68,14 @@ def _cuda(t: torch.Tensor) -> torch.device:
 
 def _call(name: str, device: torch.device, *args) -> None:
     # torch's raw handle of the current stream: the public Stream object costs 2 us to build, a
-    # tenth of a small call
+    # fifth of a small call
     index = device.index
-    if index == torch.cuda.current_device():
-        rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == torch._C._cuda_getDevice():
+        rc = getattr(lib(), name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc != _lib.RT_OK:
+            rc = getattr(lib(), name)(*args, _raw_stream(index))
+    if rc:
         raise RustaneError(rc, name)
 
 
@@ -128,7 +133,8 @@ class KvCache:
                 _fail("k_scale, v_scale: contiguous fp32 [num_pages, kv_heads, page_size]")
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, device
         self.num_pages, self.kv_heads, self.page_size, self.hd = k.shape
-        self.err = torch.zeros(1, dtype=torch.int32, device=device)
+        self.scale = 1.0 / math.sqrt(self.hd)  # of attention scores, by default
+        self.err = torch.zeros(1, dtype=_I32, device=device)
         self.err_ptr = self.err.data_ptr()
         self.c = RtKvPages(k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), self.num_pages, self.page_size,
                            self.kv_heads, self.hd, int(int8))
@@ -163,17 +169,18 @@ def _gammas(gamma_q, gamma_k, hd, device):
     if (gamma_q is None) != (gamma_k is None):
         _fail("gamma_q and gamma_k: both or neither")
     if gamma_q is not None:
-        _vec("gamma_q", gamma_q, hd, torch.float32, device)
-        _vec("gamma_k", gamma_k, hd, torch.float32, device)
+        _vec("gamma_q", gamma_q, hd, _F32, device)
+        _vec("gamma_k", gamma_k, hd, _F32, device)
 
 
 def _vectors(t: torch.Tensor, heads: int, kv_heads: int) -> tuple[int, int]:
     """(hd, v heads) of q | k | v rows: hd from the column count, with or without the v part (the count
     fits one of the four: 128 without v would be 64 with v only for heads == 0)."""
-    for hd in (64, 128):
-        for v in (kv_heads, 0):
-            if t.dim() == 2 and t.shape[1] == (heads + kv_heads + v) * hd:
-                return hd, v
+    cols = t.shape[-1] if t.dim() == 2 else 0
+    for v in (kv_heads, 0):
+        hd, rest = divmod(cols, max(1, heads + kv_heads + v))
+        if not rest and (hd == 128 or hd == 64):
+            return hd, v
     _fail(f"rows of {tuple(t.shape)} do not hold {heads} q and {kv_heads} k (and v) heads of 64 or 128")
 
 
@@ -185,15 +192,15 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, rope: Rope, heads: 
     device = _cuda(qkv)
     hd, nv = _vectors(qkv, heads, kv_heads)
     T, cols = qkv.shape
-    ld = _rows("qkv", qkv, cols, torch.bfloat16, device)
-    _vec("positions", positions, T, torch.int32, device)
+    ld = _rows("qkv", qkv, cols, _BF16, device)
+    _vec("positions", positions, T, _I32, device)
     _gammas(gamma_q, gamma_k, hd, device)
     if rope.device != device:
         _fail(f"rope: its tables have to be on {device}")
     if out is None:
-        out, ldo = qkv.new_empty((T, cols)), cols
+        out, ldo = torch.empty_like(qkv, memory_format=_DENSE), cols
     else:
-        ldo = _rows("out", out, cols, torch.bfloat16, device, T)
+        ldo = _rows("out", out, cols, _BF16, device, T)
     _call("rt_kernel_qk_norm_rope_fwd", device, qkv.data_ptr(), ld, out.data_ptr(), ldo, positions.data_ptr(),
           rope.ref, _ptr(gamma_q), _ptr(gamma_k), eps, T, heads, kv_heads, nv, hd, _ptr(err))
     return out
@@ -208,26 +215,26 @@ def qk_norm_rope_backward(dout: torch.Tensor, qkv: torch.Tensor | None, position
     device = _cuda(dout)
     hd, nv = _vectors(dout, heads, kv_heads)
     T, cols = dout.shape
-    ld = _rows("dout", dout, cols, torch.bfloat16, device)
-    _vec("positions", positions, T, torch.int32, device)
+    ld = _rows("dout", dout, cols, _BF16, device)
+    _vec("positions", positions, T, _I32, device)
     _gammas(gamma_q, gamma_k, hd, device)
     if rope.device != device:
         _fail(f"rope: its tables have to be on {device}")
     if dqkv is None:
-        dqkv, lddx = dout.new_empty((T, cols)), cols
+        dqkv, lddx = torch.empty_like(dout, memory_format=_DENSE), cols
     else:
-        lddx = _rows("dqkv", dqkv, cols, torch.bfloat16, device, T)
+        lddx = _rows("dqkv", dqkv, cols, _BF16, device, T)
     accumulate, partials, ldx = 0, None, 0
     if gamma_q is not None:
         if qkv is None:
             _fail("the gammas' backward reads qkv")
-        ldx = _rows("qkv", qkv, cols, torch.bfloat16, device, T)
+        ldx = _rows("qkv", qkv, cols, _BF16, device, T)
         if (dgamma_q is None) != (dgamma_k is None):
             _fail("dgamma_q and dgamma_k: both or neither")
         accumulate = int(dgamma_q is not None)
         if accumulate:
-            _vec("dgamma_q", dgamma_q, hd, torch.float32, device)
-            _vec("dgamma_k", dgamma_k, hd, torch.float32, device)
+            _vec("dgamma_q", dgamma_q, hd, _F32, device)
+            _vec("dgamma_k", dgamma_k, hd, _F32, device)
         else:
             dgamma_q, dgamma_k = torch.empty_like(gamma_q), torch.empty_like(gamma_k)
         partials = gamma_q.new_empty(lib().rt_kernel_qk_norm_rope_bwd_partials(T, heads, kv_heads) * hd)
@@ -242,16 +249,16 @@ def kv_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, r
     """qk_norm_rope that writes k and v of token t into cache slot slots[t] (-1: nowhere) and returns q."""
     device = cache.device
     T, hd = qkv.shape[0], cache.hd
-    ld = _rows("qkv", qkv, (heads + 2 * cache.kv_heads) * hd, torch.bfloat16, device)
-    _vec("positions", positions, T, torch.int32, device)
-    _vec("slots", slots, T, torch.int32, device)
+    ld = _rows("qkv", qkv, (heads + 2 * cache.kv_heads) * hd, _BF16, device)
+    _vec("positions", positions, T, _I32, device)
+    _vec("slots", slots, T, _I32, device)
     _gammas(gamma_q, gamma_k, hd, device)
     if rope.device != device:
         _fail(f"rope: its tables have to be on {device}")
     if q_out is None:
         q_out, ldq = qkv.new_empty((T, heads * hd)), heads * hd
     else:
-        ldq = _rows("q_out", q_out, heads * hd, torch.bfloat16, device, T)
+        ldq = _rows("q_out", q_out, heads * hd, _BF16, device, T)
     _call("rt_kernel_kv_append", device, qkv.data_ptr(), ld, q_out.data_ptr(), ldq, positions.data_ptr(),
           slots.data_ptr(), rope.ref, _ptr(gamma_q), _ptr(gamma_k), eps, cache.ref, T, heads, cache.err_ptr)
     return q_out
@@ -261,10 +268,10 @@ def kv_gather(cache: KvCache, slots: torch.Tensor, k_out: torch.Tensor | None = 
               v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Cached tokens back as bf16: (k, v) [T, kv_heads, hd]; slot -1 gives zeros."""
     device, T = cache.device, slots.shape[0]
-    _vec("slots", slots, T, torch.int32, device)
+    _vec("slots", slots, T, _I32, device)
     shape = (T, cache.kv_heads, cache.hd)
     given = [x for x in (("k_out", k_out), ("v_out", v_out)) if x[1] is not None]
-    k_out = torch.empty(shape, dtype=torch.bfloat16, device=device) if k_out is None else k_out
+    k_out = torch.empty(shape, dtype=_BF16, device=device) if k_out is None else k_out
     v_out = torch.empty_like(k_out) if v_out is None else v_out
     for name, t in given:
         if t.shape != shape or t.dtype != torch.bfloat16 or t.device != device or not t.is_contiguous():
@@ -283,20 +290,20 @@ def attention_paged(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, k
     Returns (out [T, heads * hd] bf16, lse2 [T, heads] fp32 or None)."""
     device, T, n = cache.device, q.shape[0], kv_lens.shape[0]
     cols = heads * cache.hd
-    ldq = _rows("q", q, cols, torch.bfloat16, device)
-    _vec("kv_lens", kv_lens, n, torch.int32, device)
-    _vec("q_start", q_start, n + 1, torch.int32, device)
-    ldt = _rows("page_table", page_table, page_table.shape[-1], torch.int32, device, n)
+    ldq = _rows("q", q, cols, _BF16, device)
+    _vec("kv_lens", kv_lens, n, _I32, device)
+    _vec("q_start", q_start, n + 1, _I32, device)
+    ldt = _rows("page_table", page_table, page_table.shape[-1], _I32, device, n)
     if out is None:
-        out, ldo = q.new_empty((T, cols)), cols
+        out, ldo = torch.empty_like(q, memory_format=_DENSE), cols
     else:
-        ldo = _rows("out", out, cols, torch.bfloat16, device, T)
+        ldo = _rows("out", out, cols, _BF16, device, T)
     if workspace.device != device:
         _fail(f"workspace: has to be on {device}")
-    lse2 = torch.empty((T, heads), device=device) if want_lse else None
+    lse2 = q.new_empty((T, heads), dtype=_F32) if want_lse else None
     _call("rt_kernel_attention_paged", device, q.data_ptr(), ldq, out.data_ptr(), ldo, _ptr(lse2), cache.ref,
           page_table.data_ptr(), ldt, kv_lens.data_ptr(), q_start.data_ptr(), n, T, max_q, max_kv, heads, window,
-          1.0 / math.sqrt(cache.hd) if scale is None else scale, workspace.ptr, workspace.size,
+          cache.scale if scale is None else scale, workspace.ptr, workspace.size,
           cache.err_ptr)
     return out, lse2
 
@@ -314,37 +321,37 @@ def logits_adjust(logits: torch.Tensor, hist: torch.Tensor | None = None, hist_s
     if logits.dim() != 2:
         _fail("logits: [B, V]")
     B, V = logits.shape
-    ldl = _rows("logits", logits, V, torch.float32, device)
+    ldl = _rows("logits", logits, V, _F32, device)
     r = RtLogitRules()
     if hist is not None:
         if hist_start is None:
             _fail("hist needs hist_start")
-        _vec("hist", hist, None, torch.int32, device)
-        _vec("hist_start", hist_start, B + 1, torch.int32, device)
+        _vec("hist", hist, None, _I32, device)
+        _vec("hist_start", hist_start, B + 1, _I32, device)
         r.hist, r.hist_start, r.n_hist = hist.data_ptr(), hist_start.data_ptr(), hist.shape[0]
         if n_prompt is not None:
-            _vec("n_prompt", n_prompt, B, torch.int32, device)
+            _vec("n_prompt", n_prompt, B, _I32, device)
             r.n_prompt = n_prompt.data_ptr()
     for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
         if t is not None:
-            _vec(name, t, B, torch.float32, device)
+            _vec(name, t, B, _F32, device)
             setattr(r, name, t.data_ptr())
     if bias_ids is not None:
         if bias_vals is None or bias_start is None:
             _fail("bias_ids needs bias_vals and bias_start")
-        _vec("bias_ids", bias_ids, None, torch.int32, device)
-        _vec("bias_vals", bias_vals, bias_ids.shape[0], torch.float32, device)
-        _vec("bias_start", bias_start, B + 1, torch.int32, device)
+        _vec("bias_ids", bias_ids, None, _I32, device)
+        _vec("bias_vals", bias_vals, bias_ids.shape[0], _F32, device)
+        _vec("bias_start", bias_start, B + 1, _I32, device)
         r.bias_ids, r.bias_vals, r.bias_start, r.n_bias = (bias_ids.data_ptr(), bias_vals.data_ptr(), bias_start.data_ptr(),
                                                            bias_ids.shape[0])
     if mask is not None:
-        r.mask_ld = _rows("mask", mask, (V + 31) // 32, torch.int32, device, B)
+        r.mask_ld = _rows("mask", mask, (V + 31) // 32, _I32, device, B)
         r.mask = mask.data_ptr()
     if out is None:
-        out, ldo = logits.new_empty((B, V)), V
+        out, ldo = torch.empty_like(logits, memory_format=_DENSE), V
     else:
-        ldo = _rows("out", out, V, torch.float32, device, B)
-    token = torch.empty(B, dtype=torch.int32, device=device)
+        ldo = _rows("out", out, V, _F32, device, B)
+    token = torch.empty(B, dtype=_I32, device=device)
     _call("rt_kernel_logits_adjust", device, logits.data_ptr(), ldl, out.data_ptr(), ldo, token.data_ptr(), B, V,
           ctypes.byref(r), _ptr(err))
     return out, token

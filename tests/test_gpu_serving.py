@@ -465,6 +465,25 @@ def test_attention_infinite_and_lowest_scores(n):
     close(lse, l, 1e-4 + 1e-5 * torch.where(l.isfinite(), l.abs(), 0))
 
 
+@pytest.mark.parametrize("n", [1, 2, 150])
+@pytest.mark.parametrize("q_amp,v_lo,v_hi", [(1.0, -12, 12), (2.0**40, -20, 0), (2.0**-30, 0, 30), (0.0, -60, -60), (1.0, 40, 40)])
+def test_attention_int8_rows_of_very_different_scales(n, q_amp, v_lo, v_hi):
+    """k and v rows whose scales differ by powers of two, up and down along the keys, and q far from 1: the
+    scores stay ordinary (k's scale undoes q's), the weighted rows of v span the whole range."""
+    p = Paged([n], [700], 4, 2, 128, 16, True, seed=31)
+    where = (p.table[0, :44].long()[:, None] * 16 + torch.arange(16, device="cuda")).reshape(-1)[:700]
+    page, off = where // 16, where % 16
+    step = (torch.arange(700, device="cuda") * 37 % 101).double() / 100
+    up = torch.exp2((v_lo + (v_hi - v_lo) * step).round())
+    p.q.mul_(q_amp)
+    if q_amp:
+        p.cache.k_scale[page, :, off] /= q_amp
+        p.k[0] /= q_amp
+    p.cache.v_scale[page, :, off] *= up[:, None].float()
+    p.v[0] *= up[:, None, None]
+    p.check()
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("n,H,Hk", [(3, 2, 2), (4, 8, 1), (150, 2, 2)])
 def test_attention_nonfinite_values_of_later_keys_stay_masked(n, H, Hk, bad):
