@@ -4,7 +4,9 @@ Every `.cu` / `.cpp` file under ``rustane_b200/csrc`` is compiled by nvcc for
 ``-gencode arch=compute_100a,code=sm_100a`` and linked into
 ``rustane_b200/librustane_cuda.so`` with the static CUDA runtime.  Objects are
 cached under ``rustane_b200/_build`` and rebuilt when a source or header is
-newer.  No GPU is needed to build.
+newer.  ``rustane_b200/csrc_torch/ops.cpp`` (the torch binding of the serving
+operators) is compiled by the host compiler against the installed torch into
+``rustane_b200/_torch_ops<suffix>.so``.  No GPU is needed to build.
 """
 from __future__ import annotations
 
@@ -13,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -20,6 +23,8 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "librustane_cuda.so"
 INCLUDE = PKG.parent / "include"
+TORCH_SRC = PKG / "csrc_torch" / "ops.cpp"
+TORCH_EXT = PKG / f"_torch_ops{sysconfig.get_config_var('EXT_SUFFIX')}"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -53,6 +58,28 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def build_torch_ext(verbose: bool = False) -> Path:
+    """The torch binding; links librustane_cuda.so (found next to it at run time)."""
+    newest = max([TORCH_SRC.stat().st_mtime] + [h.stat().st_mtime for h in INCLUDE.glob("*.h")])
+    if TORCH_EXT.exists() and TORCH_EXT.stat().st_mtime >= newest:
+        return TORCH_EXT
+    import torch
+    root = Path(torch.__file__).parent
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda, INCLUDE,
+           sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_torch_ops",
+           *(f"-isystem{i}" for i in inc), str(TORCH_SRC), "-o", str(TORCH_EXT), f"-L{PKG}", "-l:librustane_cuda.so",
+           f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {TORCH_SRC.name}:\n{res.stdout}\n{res.stderr}")
+    return TORCH_EXT
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
     BUILD.mkdir(exist_ok=True)
     sources = sorted(list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cpp")))
@@ -67,6 +94,7 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    build_torch_ext(verbose)
     return LIB
 
 
