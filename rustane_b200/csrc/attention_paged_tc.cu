@@ -84,6 +84,16 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
                  "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
                  "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
+// One lane of a converged warp, and a value that all its lanes share, in the forms that the
+// compiler keeps in uniform registers: tcgen05.mma takes its operands from there, and moving them
+// over for every product took one lane 100 clocks a product.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 __device__ __forceinline__ void softmax_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 // the two softmax warps (one a stream) of TMEM lane quadrant qw
 __device__ __forceinline__ void quad_bar(int qw) { asm volatile("bar.sync %0, 64;" ::"r"(2 + qw) : "memory"); }
@@ -294,15 +304,20 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
     // ------------------------------------------------------- MMA issuer of stream u
     constexpr uint32_t idesc_s = idesc_bf16_f32(kBM, kSub, false, false);  // Q, K: both hd-contiguous
     constexpr uint32_t idesc_o = idesc_bf16_f32(kBM, HD, false, true);    // P key-contiguous, V hd-contiguous
-    const int u = warp >> 1;
-    const uint32_t ts = tmem + u * 128, to = tmem + 256 + u * 128;
+    const int u = uniform(warp >> 1);
+    const uint32_t ts = uniform(tmem) + u * 128, to = uniform(tmem) + 256 + u * 128;
+    // Descriptors of the first tile; others are a number of 16-byte units further (building one for
+    // every product took one lane longer than the products themselves)
+    const uint64_t q_desc = smem_desc_sw128(smem_u32(smem + C::Q), 16, 1024);
+    const uint64_t kv_desc = smem_desc_sw128(smem_u32(smem + C::KV), 16, 1024);
+    const uint64_t v_desc = smem_desc_sw128(smem_u32(smem + C::KV), kAtomBytes, 1024);
     bool ok = true;
     int g = 0, it = 0, n = 0;  // n: 64-key steps of this stream so far
     for (; ok && w.more(); w.next()) {
       if (w.empty()) continue;
       const int cnt = w.count();
       const Share sh(w, half);
-      const uint32_t sq = smem_u32(smem + C::Q + (sh.pair ? u * C::TILE : 0));
+      const uint64_t dq = q_desc + uniform(sh.pair ? u * (C::TILE >> 4) : 0);
       if (!wait_all(&bar[kQFull], it & 1)) {
         ok = false;
         break;
@@ -328,17 +343,19 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
             (nn >= 2 && !wait_all(&bar[kPvDone + 2 * u + (nn & 1)], ((nn - 2) >> 1) & 1)))
           return false;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t sk = smem_u32(smem + C::KV + kx * C::TILE) + h * (kSub * 128);
+        const uint64_t dk = kv_desc + uniform(kx * (C::TILE >> 4) + h * (kSub * 128 >> 4));
+        const uint32_t buf = uniform(nn & 1);
+        const bool free_k = uniform(h == 1), free_q = uniform(h == 1 && sh.ends(u, bb, cnt));
+        const uint32_t k_slot = uniform(kx);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * kAtomBytes + (kk & 3) * 32;
-            umma_bf16(ts + (nn & 1) * kSub, smem_desc_sw128(sq + off, 16, 1024), smem_desc_sw128(sk + off, 16, 1024),
-                      idesc_s, kk != 0 ? 1u : 0u);
+            const uint32_t off = ((kk >> 2) * kAtomBytes + (kk & 3) * 32) >> 4;
+            umma_bf16(ts + buf * kSub, dq + off, dk + off, idesc_s, kk != 0 ? 1u : 0u);
           }
-          umma_commit(&bar[kSFull + 2 * u + (nn & 1)]);
-          if (h == 1) umma_commit(&bar[kTileEmpty + kx]);
-          if (h == 1 && sh.ends(u, bb, cnt)) umma_commit(&bar[kQEmpty]);
+          umma_commit(&bar[kSFull + 2 * u + buf]);
+          if (free_k) umma_commit(&bar[kTileEmpty + k_slot]);
+          if (free_q) umma_commit(&bar[kQEmpty]);
         }
         __syncwarp();
         return true;
@@ -383,14 +400,15 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
                (!first || it == 0 || wait_all(&bar[kOFree], (it - 1) & 1));
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t sv = smem_u32(vt) + h * (kSub * 128);
+          const uint64_t dv = v_desc + uniform(vx * (C::TILE >> 4) + h * (kSub * 128 >> 4));
+          const uint32_t buf = uniform(n & 1), v_slot = uniform(vx);
+          const bool free_v = uniform(h == 1), add0 = uniform(!first);
+          if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < kSub / 16; ++kk)
-              umma_bf16_ts(to, ts + (n & 1) * kSub + kk * 8, smem_desc_sw128(sv + kk * 2048, kAtomBytes, 1024), idesc_o,
-                           first && kk == 0 ? 0u : 1u);
-            umma_commit(&bar[kPvDone + 2 * u + (n & 1)]);
-            if (h == 1) umma_commit(&bar[kTileEmpty + vx]);
+              umma_bf16_ts(to, ts + buf * kSub + kk * 8, dv + kk * (2048 >> 4), idesc_o, kk == 0 && !add0 ? 0u : 1u);
+            umma_commit(&bar[kPvDone + 2 * u + buf]);
+            if (free_v) umma_commit(&bar[kTileEmpty + v_slot]);
           }
           __syncwarp();
           first = false;
@@ -409,7 +427,7 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
       if (lane == 0) set_error(a.err, kDevTimeoutMma);
       *abort_flag = 1;
     }
-    if (lane == 0) {
+    if (elect_one()) {  // the lane that issued the products
       umma_commit(&bar[kDrain + u]);
       mbar_wait(&bar[kDrain + u], 0);
     }
