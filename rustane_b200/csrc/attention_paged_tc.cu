@@ -448,10 +448,13 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
         for (int r = threadIdx.x - 384; r < kBK; r += 64) {  // keys of the block
           const uint8_t* src = smem + C::CODE + cs * C::CODES + r * C::ROW8;
           uint8_t* dst = smem + C::KV + st * C::TILE + r * 128;
+          uint4 codes[HD / 16];  // all of the key's first: the compiler moves no load before a store
+#pragma unroll
+          for (int ch = 0; ch < HD / 16; ++ch)
+            codes[ch] = *reinterpret_cast<const uint4*>(src + (HD == 64 ? ch ^ ((r >> 1) & 3) : ch ^ (r & 7)) * 16);
 #pragma unroll
           for (int ch = 0; ch < HD / 16; ++ch) {
-            const int sw = HD == 64 ? ch ^ ((r >> 1) & 3) : ch ^ (r & 7);
-            const uint4 q = *reinterpret_cast<const uint4*>(src + sw * 16);
+            const uint4 q = codes[ch];
             uint8_t* d = dst + (ch >> 2) * kAtomBytes;
             const int c0 = (ch & 3) * 2;
             *reinterpret_cast<uint4*>(d + ((c0 ^ (r & 7)) << 4)) =
