@@ -16,9 +16,8 @@
 //   warp 2      owns the TMEM allocation;
 //   warps 4-11  softmax, 4 warps a stream: the row's maximum, then P; O rescaled only when the
 //               running maximum grew by more than 2^8;
-//   warps 12, 13 (int8 cache) turn the codes into bf16 tiles, exactly, two keys a thread (four
-//               warps of one key a thread were 9% slower on long chunks: they took issue slots);
-//               k's scale multiplies the scores and v's the weights, in fp32.
+//   warps 12-15 (int8 cache) turn the codes into bf16 tiles, exactly, one key a thread; k's scale
+//               multiplies the scores and v's the weights, in fp32.
 // (One stream of two threads a row measured 525 TFLOP/s on 4 x 509 tokens over up to 4091; two
 // streams with one S buffer of 128 keys each waited 2300 of 5600 clocks for their next S.)
 // P is rounded to bf16 for the P V product (its sum is not).  All waits are bounded.
@@ -72,7 +71,7 @@ struct Cfg {
   static constexpr int NANS = ML + 2 * kBM * 8;                             // unsigned [4 quadrants][2 streams]
   static constexpr int BAR = NANS + 64;
   static constexpr int BYTES = BAR + 512 + 1024;
-  static constexpr int THREADS = I8 ? 448 : 384;
+  static constexpr int THREADS = I8 ? 512 : 384;
 };
 static_assert(kNumBars * 8 + 16 <= 512, "barrier area");
 
@@ -171,12 +170,12 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
       mbar_init(&bar[kPvDone + i], 1);
     }
     for (int i = 0; i < C::RING; ++i) {
-      mbar_init(&bar[kTileFull + i], I8 ? 2 : 1);
+      mbar_init(&bar[kTileFull + i], I8 ? 4 : 1);
       mbar_init(&bar[kTileEmpty + i], 2);
     }
     for (int i = 0; i < kStages8; ++i) {
       mbar_init(&bar[kCodeFull + i], 1);
-      mbar_init(&bar[kCodeEmpty + i], 2);
+      mbar_init(&bar[kCodeEmpty + i], 4);
     }
     for (int i = 0; i < kScaleSlots; ++i) {
       mbar_init(&bar[kScaleFull + i], 1);
@@ -445,7 +444,8 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
         const int cs = x % kStages8, st = x % C::RING;
         ok = wait_all(&bar[kCodeFull + cs], (x / kStages8) & 1) && wait_all(&bar[kTileEmpty + st], ((x / C::RING) & 1) ^ 1);
         if (!ok) break;
-        for (int r = threadIdx.x - 384; r < kBK; r += 64) {  // keys of the block
+        {
+          const int r = threadIdx.x - 384;  // key of the block
           const uint8_t* src = smem + C::CODE + cs * C::CODES + r * C::ROW8;
           uint8_t* dst = smem + C::KV + st * C::TILE + r * 128;
           uint4 codes[HD / 16];  // all of the key's first: the compiler moves no load before a store
@@ -536,25 +536,17 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
           tc_fence_after();
           uint32_t v[2][32];
           const int last = hi_r - key0, from = lo_r - key0;  // seen: from <= e < last
-          auto finish = [&](uint32_t (&x)[32], int c) {  // k's scale (int8), -inf where unseen
-            if (I8) {
+          auto scale_k = [&](uint32_t (&x)[32], int c) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                const float4 k4 = *reinterpret_cast<const float4*>(scales + c * 32 + e);
-                float x0, x1, x2, x3;
-                f2_unpack(f2_mul(f2_pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2_pack(k4.x, k4.y)), x0, x1);
-                f2_unpack(f2_mul(f2_pack(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), f2_pack(k4.z, k4.w)), x2,
-                          x3);
-                x[e] = __float_as_uint(x0);
-                x[e + 1] = __float_as_uint(x1);
-                x[e + 2] = __float_as_uint(x2);
-                x[e + 3] = __float_as_uint(x3);
-              }
-            }
-            if (masked) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (c * 32 + e >= last || c * 32 + e < from) x[e] = __float_as_uint(-CUDART_INF_F);
+            for (int e = 0; e < 32; e += 4) {
+              const float4 k4 = *reinterpret_cast<const float4*>(scales + c * 32 + e);
+              float x0, x1, x2, x3;
+              f2_unpack(f2_mul(f2_pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2_pack(k4.x, k4.y)), x0, x1);
+              f2_unpack(f2_mul(f2_pack(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), f2_pack(k4.z, k4.w)), x2, x3);
+              x[e] = __float_as_uint(x0);
+              x[e + 1] = __float_as_uint(x1);
+              x[e + 2] = __float_as_uint(x2);
+              x[e + 3] = __float_as_uint(x3);
             }
           };
           auto top = [](const uint32_t (&x)[32]) {
@@ -572,8 +564,15 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
           tmem_ld32(ts + 32, v[1]);
           tmem_ld_wait(v[0]);
           tmem_ld_wait(v[1]);
-          finish(v[0], 0);
-          finish(v[1], 1);
+          if (I8) {
+            scale_k(v[0], 0);
+            scale_k(v[1], 1);
+          }
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if (e >= last || e < from) v[e >> 5][e & 31] = __float_as_uint(-CUDART_INF_F);
+          }
           const float m_new = fmax3(m_used, top(v[0]), top(v[1]));
           if (first) {
             m_used = m_new;
@@ -623,11 +622,6 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
                 const float4 vs = *reinterpret_cast<const float4*>(scales + kBK + c * 32 + e);
                 f2_unpack(f2_mul(f2_pack(pw[0], pw[1]), f2_pack(vs.x, vs.y)), pw[0], pw[1]);
                 f2_unpack(f2_mul(f2_pack(pw[2], pw[3]), f2_pack(vs.z, vs.w)), pw[2], pw[3]);
-                if (masked) {  // 0 whatever the scale of an unseen key is
-#pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    if (x[e + i] == 0xff800000u) pw[i] = 0.f;
-                }
               }
               pk[e / 2] = pack_bf16x2(pw[0], pw[1]);
               pk[e / 2 + 1] = pack_bf16x2(pw[2], pw[3]);
@@ -641,6 +635,18 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
             l += (a0 + a1) + (b0 + b1);
           }
           tmem_st_wait();
+          if (I8 && masked) {
+            // 0 where unseen, whatever the scale of that key is (a branch in the loop above, which
+            // keeps the compiler from mixing its two halves, cost every step 13%)
+            uint32_t pw[32];
+            tmem_ld32(ts, pw);
+            tmem_ld_wait(pw);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              pw[i] &= (2 * i >= from && 2 * i < last ? 0xffffu : 0u) | (2 * i + 1 >= from && 2 * i + 1 < last ? 0xffff0000u : 0u);
+            tmem_st32(ts, pw);
+            tmem_st_wait();
+          }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar[kPFull + 2 * u + (n & 1)]);
