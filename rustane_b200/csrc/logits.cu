@@ -15,11 +15,13 @@
 // tokens at a time and every CTA reads the row's whole history (4 bytes a token, from L2
 // after the first CTA) into them with integer atomics, whose order does not change the
 // counts.  The CTAs' best tokens meet in the first CTA's shared memory.
-// 192 rows of 128003 with 2000 history tokens and 40 biases each: 88 us, 2.3 TB/s of the 8 bytes a
-// logit (53 us with neither, 46 without counts): parts of 8192 tokens alternate counting,
+// 192 rows of 128003 with 2000 history tokens and 40 biases each: 82 us, 2.4 TB/s of the 8 bytes a
+// logit (55 us with neither, 46 without counts): parts of 8192 tokens alternate counting,
 // streaming and biases between barriers, and half of all issue slots go to the penalties of
-// vectors that hold a listed token.  A list of the touched tokens that does the penalties after
-// the streaming took 97 us, whole waves of 3 CTAs a row 121, 128 threads a CTA 89 to 119.
+// vectors that hold a listed token.  Biases and the first history tokens are fetched ahead (89 us
+// without; 8 tokens a thread instead of 4: 87).  A list of the touched tokens that does the
+// penalties after the streaming took 97 us, whole waves of 3 CTAs a row 121, 128 threads a CTA 89
+// to 119, branch-free penalties 93.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -53,6 +55,7 @@ struct Params {
   int slice;  // places per CTA, a multiple of 128
 };
 
+constexpr int kHist = 4;   // history tokens in flight per thread
 constexpr int kBatch = 4;  // 16-byte loads (or 4-byte ones, VEC false) in flight per thread
 
 // VEC: the rows of in and out are equally far from a 16-byte boundary, so both take 16-byte
@@ -61,6 +64,8 @@ constexpr int kBatch = 4;  // 16-byte loads (or 4-byte ones, VEC false) in fligh
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const Params p) {
   extern __shared__ uint32_t cnt[];
+  __shared__ int32_t held_ids[kThreads];
+  __shared__ float held_vals[kThreads];
   __shared__ Best warp_best[kThreads / 32];
   __shared__ Best cta_best[8];  // of the cluster's CTAs, in the first one
   const LogitsArgs& a = p.a;
@@ -114,28 +119,51 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const Params
   };
   if (VEC) load(lo_all + 4 * tid);
 
+  // The thread's first history tokens (every part starts with them) and the row's biases, fetched
+  // before anything waits.
+  int id0[kHist];
+  auto fetch = [&](int64_t j0, int (&id)[kHist]) {  // -1: no token
+#pragma unroll
+    for (int u = 0; u < kHist; ++u) id[u] = j0 + u * kThreads < h1 ? a.hist[j0 + u * kThreads] : -1;
+  };
+  fetch(h0 + tid, id0);
+  const int32_t* bias_ids = a.bias_ids + b0;
+  const float* bias_vals = a.bias_vals + b0;
+  const int64_t nb = b1 - b0;
+  if (nb > 0 && nb <= kThreads) {
+    if (tid < nb) {
+      held_ids[tid] = bias_ids[tid];
+      held_vals[tid] = bias_vals[tid];
+    }
+    bias_ids = held_ids;
+    bias_vals = held_vals;
+  }
+
   for (int lo = lo_all; lo < hi_all; lo += kSub) {
     const int hi = min(hi_all, lo + kSub), n = hi - lo;
     const int id_lo = lo - shift, id_hi = hi - shift;  // tokens of these places
     if (counted) {
       for (int i = 4 * tid; i < n; i += 4 * kThreads) *reinterpret_cast<uint4*>(cnt + i) = make_uint4(0, 0, 0, 0);
       __syncthreads();
-      for (int64_t j0 = h0 + tid; j0 < h1; j0 += kBatch * kThreads) {
-        int id[kBatch];
+      auto count = [&](int64_t j0, const int (&id)[kHist]) {
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) id[u] = j0 + u * kThreads < h1 ? a.hist[j0 + u * kThreads] : id_hi;
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const int64_t j = j0 + u * kThreads;
-          if (j < h1 && (id[u] < -1 || id[u] >= a.V)) set_error(a.err, kDevBadToken);
-          else if (id[u] >= max(id_lo, 0) && id[u] < id_hi && j < h1) {
-            if (j < made0) atomicOr(&cnt[id[u] - id_lo], kSeen);
+        for (int u = 0; u < kHist; ++u) {
+          if (static_cast<unsigned>(id[u]) >= static_cast<unsigned>(a.V)) {
+            if (id[u] != -1) set_error(a.err, kDevBadToken);
+          } else if (static_cast<unsigned>(id[u] - id_lo) < static_cast<unsigned>(n)) {
+            if (j0 + u * kThreads < made0) atomicOr(&cnt[id[u] - id_lo], kSeen);
             else atomicAdd(&cnt[id[u] - id_lo], 1u);
           }
         }
+      };
+      if (h0 + tid < h1) count(h0 + tid, id0);
+      for (int64_t j0 = h0 + tid + kHist * kThreads; j0 < h1; j0 += kHist * kThreads) {
+        int id[kHist];
+        fetch(j0, id);
+        count(j0, id);
       }
-      for (int64_t j = b0 + tid; j < b1; j += kThreads) {
-        const int id = a.bias_ids[j];
+      for (int64_t j = tid; j < nb; j += kThreads) {
+        const int id = bias_ids[j];
         if (id < -1 || id >= a.V) set_error(a.err, kDevBadToken);
         else if (id >= max(id_lo, 0) && id < id_hi) atomicOr(&cnt[id - id_lo], kBiased);
       }
@@ -216,17 +244,17 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const Params
           if (x0 + u * kThreads < hi) one(x0 + u * kThreads, raw[u]);
       }
     }
-    if (b1 > b0) {
+    if (nb > 0) {
       __syncthreads();
       if (tid < 32) {
         // 32 entries at a time in list order; lanes with the same token add up one after another
-        for (int64_t base = b0; base < b1; base += 32) {
+        for (int64_t base = 0; base < nb; base += 32) {
           const int64_t j = base + tid;
           int id = -1;
           float val = 0.f;
-          if (j < b1) {
-            id = a.bias_ids[j];
-            val = a.bias_vals[j];
+          if (j < nb) {
+            id = bias_ids[j];
+            val = bias_vals[j];
             if (id < max(id_lo, 0) || id >= id_hi) id = -1;
           }
           const uint32_t same = __match_any_sync(0xffffffffu, id);
@@ -243,8 +271,8 @@ __global__ void __launch_bounds__(kThreads, 4) logits_adjust_kernel(const Params
         }
       }
       __syncthreads();
-      for (int64_t j = b0 + tid; j < b1; j += kThreads) {  // entries of one token write the same value
-        const int id = a.bias_ids[j];
+      for (int64_t j = tid; j < nb; j += kThreads) {  // entries of one token write the same value
+        const int id = bias_ids[j];
         if (id < max(id_lo, 0) || id >= id_hi) continue;
         float l = __uint_as_float(cnt[id - id_lo]);
         if (!allowed(id)) l = -INFINITY;
