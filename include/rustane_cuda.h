@@ -480,7 +480,7 @@ RT_API int rt_kernel_kv_gather(const rt_kv_pages* cache, const int32_t* slots, v
  * q_start[s + 1]) (q_start[nseq + 1] ascending from 0 to T) and the first kv_lens[s] tokens
  * of its pages page_table[s * table_ld + ..], the new tokens (already appended) last: row i
  * of n sits at position kv_lens[s] - n + i and sees the keys up to its own, the last
- * `window` of them if window > 0.  A row that sees none gives out = 0, lse2 = -inf.  lse2
+ * `window` of them if window > 0; scale > 0.  A row that sees none gives out = 0, lse2 = -inf.  lse2
  * (nullable): [T, heads] log2 of the sum of exponentials.  max_q, max_kv: upper bounds of
  * the new tokens and the length of any sequence; they choose the kernel and size the grid,
  * and the work follows the device lengths.  A length outside [0, table_ld * page_size]

@@ -7,8 +7,9 @@
 // clock and SM) take as long as the products at hd 128.  One persistent CTA per SM runs two
 // streams, each with its own S and O in TMEM, its own MMA warp and its own 128 softmax
 // threads, one row each.  A stream takes 64 keys at a time, into two S buffers in turn, so the
-// scores of the next 64 are ready before the weights of the last are in the product.  An item is up to 2 x 128 rows; the streams take a half each and share every K and V
-// tile, or, if the rows fit one half, take the blocks in turn and add up at the end.
+// scores of the next 64 are ready before the weights of the last are in the product.  An item is
+// up to 2 x 128 rows; the streams take a half each and share every K and V tile, or, if the rows
+// fit one half, take the blocks in turn and add up at the end.
 //   warp 0      TMA producer: Q of each item (one box a half: whole tokens x the G heads of the
 //               key head), then the pages of 128-key K and V tiles into one ring;
 //   warps 1, 3  MMA issuers of the two streams: S_{n+1} = Q K^T, then O += P_n V with P (over
@@ -18,8 +19,13 @@
 //               running maximum grew by more than 2^8;
 //   warps 12-15 (int8 cache) turn the codes into bf16 tiles, exactly, one key a thread; k's scale
 //               multiplies the scores and v's the weights, in fp32.
-// (One stream of two threads a row measured 525 TFLOP/s on 4 x 509 tokens over up to 4091; two
-// streams with one S buffer of 128 keys each waited 2300 of 5600 clocks for their next S.)
+// Measured: 4 x 509 tokens over up to 4091, 20 heads, 102 us (597 TFLOP/s); 1024 over 8192, 16 heads,
+// 98 us (659; int8 136 us); 1531 over 20011, 32 query and 8 key heads, int8, 793 us (609).  Per 64-key step of
+// 2450 clocks the softmax waits 700 for its scores, takes 260 for the maximum and 1010 for the
+// exponentials; start-up, partial results and the join of split items are a sixth of the 102 us.
+// Other forms, same cases: one stream of two threads a row 115; one S buffer of 128 keys a
+// stream 157; S of 128 keys into both buffers 107; P in shared memory 108; exponentials partly on the FMA
+// pipe 104 and up; int8 with a branch for unseen weights inside the exponent loop +13%.
 // P is rounded to bf16 for the P V product (its sum is not).  All waits are bounded.
 #include "attention_paged.cuh"
 #include "kernels.h"

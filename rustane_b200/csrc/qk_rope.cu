@@ -20,6 +20,10 @@
 // GPU: a warp has the next group's loads in flight while it works on one, and reads a token's
 // position and tables once per run.  (Pairs exchanged by shuffles and scalar arithmetic: 17
 // instructions an entry, half of all issue slots, 4.2 TB/s on 8209 tokens of 96 heads.)
+// Measured: forward + backward of 16389 tokens of 32 + 8 + 8 heads of 128 215 us, 4.5 TB/s; append
+// of 8209 tokens of 96 heads into bf16 pages 77 us, 5.3 TB/s; gather from int8 pages 116 us, 6.4
+// TB/s, the copy rate.  16 warps an SM with one group in flight each are short of the copy rate:
+// 24 warps with the groups as they are spill (378 us), with half the group 242 us.
 #include "common.cuh"
 #include "kernels.h"
 #include "serving.h"
