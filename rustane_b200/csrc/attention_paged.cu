@@ -19,16 +19,20 @@
 // to bf16 for the P V product (its sum is not): 2^-9 of each weight.
 //
 // Measured, of the copy rate: 8 sequences of up to 40037 tokens, 32 query and 8 key heads, 176 us
-// (99%); 48 x 3000 of 16 heads 203 us (99%); 48 x up to 6011 tokens of 32 heads in int8 245 us (80%:
+// (99%); 48 x 3000 of 16 heads 203 us (99%); 48 x up to 6011 tokens of 32 heads in int8 255 us (77%:
 // the conversion's integer instructions); one sequence of 512 tokens of 12 heads 9.3 us, most of
 // it the launch and a chain of dependent loads (lengths, page, keys) and the join.
 //
 // int8: the codes become fp16, exactly (two and a half instructions a pair, one and a half of
 // them on the integer pipe; bf16 takes four and three, and that pipe was the limit: 354 us
-// for the int8 case above).  q is brought into fp16's range by one power of two
-// per item, exact down to 2^-22 of the largest entry; k's scale multiplies the score in fp32.
+// for the int8 case above).  Each row of q is brought into fp16's range by a
+// power of two, exact down to 2^-22 of its largest entry; k's scale multiplies the score in fp32.
 // The weights times v's scales are rounded to fp16 (2^-11 of each) in units of 2^kv, a power of
-// two that a warp moves, with its sums, when its largest weight leaves [2^0, 2^15) units.
+// two of each row that moves, with the row's sums, when its largest weight leaves [2^0, 2^15)
+// units.  (One power for all rows of an item lost those of much smaller q, and those before a
+// token whose v is 2^26 times larger; the int8 case took 245 us.)  A step with a key whose scale lies
+// far below a row's unit takes its small weights in further products of 2^-24 the unit each, so
+// that columns where the large keys hold zeros keep theirs.
 #include <cuda_fp16.h>
 
 #include "attention_paged.cuh"
@@ -259,30 +263,39 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
         qb[ks][t][1] = in ? x[I8 ? 1 : 4] : 0u;
       }
     }
-    float s_scale = p.scale_log2;
-    int kv = 0;  // int8: O is in units of 2^kv
+    float s_scale[NT][2];  // of rows 8 t + 2c + x
+    int kv[NT][2];         // int8: O is in units of 2^kv
+    float least = 1.f;     // the smallest 2^-kv of the thread's rows
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        s_scale[t][x] = p.scale_log2;
+        kv[t][x] = 0;
+      }
     if (I8) {
-      // the largest finite entry to [2^8, 2^9)
-      unsigned top = 0;
+      // each row's largest finite entry to [2^8, 2^9)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+      for (int t = 0; t < NT; ++t) {
+        unsigned top = 0;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const unsigned hi16 = qb[ks][t][x] >> 16 & 0x7fffu, lo16 = qb[ks][t][x] & 0x7fffu;
             top = max(top, max(hi16 < 0x7f80u ? hi16 : 0u, lo16 < 0x7f80u ? lo16 : 0u));
           }
-      top = __reduce_max_sync(0xffffffffu, top);
-      const int eq = max(-100, static_cast<int>(top >> 7) - 127 - 8);
-      const float down = power_of_2(-eq);
-      s_scale *= power_of_2(eq);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+        for (int d = 1; d < 4; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const int eq = max(-100, static_cast<int>(top >> 7) - 127 - 8);
+        const float down = power_of_2(-eq);
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int x = 0; x < 2; ++x) s_scale[t][x] *= power_of_2(__shfl_sync(0xffffffffu, eq, (2 * c + x) * 4));
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
           for (int x = 0; x < 2; ++x) qb[ks][t][x] = pack_f16x2(bf16lo(qb[ks][t][x]) * down, bf16hi(qb[ks][t][x]) * down);
+      }
     }
     // O^T of columns dg * 16 ..: entries 0, 1 (rows 8 t + 2c, + 1) of column gr (int8: 2 gr),
     // entries 2, 3 of column gr + 8 (int8: 2 gr + 1)
@@ -348,19 +361,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
         }
         // ------------------------------------------------- scale, mask, running maximum
         const bool masked = key0 < lo_all || key0 + 16 > hi_all;
-        float vs[2] = {1.f, 1.f}, ss[2] = {s_scale, s_scale};
+        float vs[2] = {1.f, 1.f}, ks2[2] = {1.f, 1.f};
         if (I8) {
           const float* sc = reinterpret_cast<const float*>(smem + st * C::SLOT + 2 * C::TILE) + warp * 16 + gr;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            ss[x] *= sc[8 * x];
+            ks2[x] = sc[8 * x];
             vs[x] = sc[kBK + 8 * x];
           }
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[t][e] *= ss[e >> 1];
+          for (int e = 0; e < 4; ++e) s[t][e] *= I8 ? s_scale[t][e & 1] * ks2[e >> 1] : p.scale_log2;
         uint32_t seen = 0xffffffffu;  // bit 4 t + e
         if (masked) {
 #pragma unroll
@@ -386,6 +399,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
             grow = grow || mx[t][x] > m[t][x] + kRescale;
           }
         const bool raised = __any_sync(0xffffffffu, grow);
+        int fell[NT][2];  // int8: a row's O fell by 2^fell or more (255: it was 0)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) fell[t][0] = fell[t][1] = 0;
         if (raised) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -394,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
             for (int x = 0; x < 2; ++x) {
               const bool gx = mx[t][x] > m[t][x] + kRescale;
               f[x] = gx ? ex2_approx(m[t][x] - mx[t][x]) : 1.f;
+              if (I8 && gx) fell[t][x] = m[t][x] == -CUDART_INF_F ? 255 : static_cast<int>(fminf(mx[t][x] - m[t][x], 255.f));
               if (gx) m[t][x] = mx[t][x];
               l[t][x] *= f[x];
             }
@@ -423,34 +440,56 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
             pb[t][1] = transpose8(pack_bf16x2(s[t][2], s[t][3]));
           }
         }
+        float y[NT][4];
+        bool wide = false;  // int8: a key's scale lies far below a row's unit
         if (I8) {
-          unsigned top = 0;  // the largest finite weight
+          auto in_units = [&] {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              const float unit[2] = {power_of_2(-kv[t][0]), power_of_2(-kv[t][1])};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[t][e] = s[t][e] * unit[e & 1];
+            }
+          };
+          in_units();
+          auto far_below = [&] {
+            return (vs[0] != 0.f && fabsf(vs[0]) * least < 0.25f) || (vs[1] != 0.f && fabsf(vs[1]) * least < 0.25f);
+          };
+          bool rare = raised || far_below();
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const unsigned x = __float_as_uint(s[t][e]) & 0x7fffffffu;
-              top = max(top, x < 0x7f800000u ? x : 0u);
+            for (int e = 0; e < 4; ++e) rare = rare || fabsf(y[t][e]) >= 32768.f;
+          if (__any_sync(0xffffffffu, rare)) {
+            // A row's unit follows its own largest finite weight: up where that leaves fp16, down where the
+            // row's O has fallen, and no further than it fell, so that O's own numbers do not grow.
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              float f[2];
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const unsigned x0 = __float_as_uint(s[t][x]) & 0x7fffffffu, x1 = __float_as_uint(s[t][2 + x]) & 0x7fffffffu;
+                unsigned top = max(x0 < 0x7f800000u ? x0 : 0u, x1 < 0x7f800000u ? x1 : 0u);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const int above = static_cast<int>(top >> 23) - 127 - kv[t][x];
+                int to = kv[t][x];
+                if (top && above >= 15) to += above - 10;
+                else if (top && above < 0) to += max(above - 10, -fell[t][x]);
+                to = max(max(-100, kv[t][x] - 120), min(120, to));
+                f[x] = ldexpf(1.f, kv[t][x] - to);
+                kv[t][x] = to;
+              }
+#pragma unroll
+              for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][t][e] *= f[e & 1];
             }
-          top = __reduce_max_sync(0xffffffffu, top);
-          const int above = static_cast<int>(top >> 23) - 127 - kv;
-          // too large for fp16, or, where the weights' own unit has just moved, small
-          if (top && (above >= 15 || (raised && above < 0))) {
-            const int to = max(max(-100, kv - 120), min(120, kv + above - 10));
-            const float f = ldexpf(1.f, kv - to);
-            kv = to;
+            in_units();
+            least = power_of_2(-kv[0][0]);
 #pragma unroll
-            for (int i = 0; i < KS; ++i)
-#pragma unroll
-              for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][t][e] *= f;
-          }
-          const float unit = power_of_2(-kv);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            pb[t][0] = transpose8(pack_f16x2(s[t][0] * unit, s[t][1] * unit));
-            pb[t][1] = transpose8(pack_f16x2(s[t][2] * unit, s[t][3] * unit));
+            for (int t = 0; t < NT; ++t) least = fminf(least, fminf(power_of_2(-kv[t][0]), power_of_2(-kv[t][1])));
+            wide = __any_sync(0xffffffffu, far_below());
           }
         }
         // ----------------------------------------------------------------- O^T += V^T P^T
@@ -482,18 +521,67 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
           }
         } else {
           const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+          auto weights = [&](const float (&z)[NT][4]) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              pb[t][0] = transpose8(pack_f16x2(z[t][0], z[t][1]));
+              pb[t][1] = transpose8(pack_f16x2(z[t][2], z[t][3]));
+            }
+          };
           // the 16 columns are taken as their even ones, then their odd ones
+          auto product = [&](auto add) {
 #pragma unroll
-          for (int dg = 0; dg < KS; dg += 2) {
-            uint32_t vb[4];
-            ldsm4t(vt + tile_off<C::ROW>(key, dg + (lane >> 4)), vb);
+            for (int dg = 0; dg < KS; dg += 2) {
+              uint32_t vb[4];
+              ldsm4t(vt + tile_off<C::ROW>(key, dg + (lane >> 4)), vb);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const uint32_t v0 = vb[2 * x] ^ 0x80808080u, v1 = vb[2 * x + 1] ^ 0x80808080u;
-              const uint32_t va[4] = {codes_f16x2<0, 2>(v0), codes_f16x2<1, 3>(v0), codes_f16x2<0, 2>(v1),
-                                      codes_f16x2<1, 3>(v1)};
+              for (int x = 0; x < 2; ++x) {
+                const uint32_t v0 = vb[2 * x] ^ 0x80808080u, v1 = vb[2 * x + 1] ^ 0x80808080u;
+                const uint32_t va[4] = {codes_f16x2<0, 2>(v0), codes_f16x2<1, 3>(v0), codes_f16x2<0, 2>(v1),
+                                        codes_f16x2<1, 3>(v1)};
 #pragma unroll
-              for (int t = 0; t < NT; ++t) mma16816h(o[dg + x][t], va, pb[t][0], pb[t][1]);
+                for (int t = 0; t < NT; ++t) add(o[dg + x][t], va, t);
+              }
+            }
+          };
+          // Weights below 2^-10 units next to larger scales: kept back here, and taken below in units
+          // of 2^-24, 2^-48, .. of the first.
+          constexpr float kSmall = 0x1p-10f;
+          float rest[NT][4];
+          if (wide) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                rest[t][e] = fabsf(y[t][e]) < kSmall ? y[t][e] : 0.f;
+                y[t][e] = rest[t][e] == 0.f ? y[t][e] : 0.f;
+              }
+          }
+          weights(y);
+          product([&](float (&d)[4], const uint32_t (&va)[4], int t) { mma16816h(d, va, pb[t][0], pb[t][1]); });
+          if (wide) {
+            float down = 1.f;
+#pragma unroll 1
+            for (int level = 1; level < 12; ++level) {
+              bool left = false;
+              down *= 0x1p-24f;
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float z = rest[t][e] * 0x1p24f;
+                  left = left || z != 0.f;
+                  rest[t][e] = fabsf(z) < kSmall ? z : 0.f;
+                  y[t][e] = rest[t][e] == 0.f ? z : 0.f;
+                }
+              if (down == 0.f || !__any_sync(0xffffffffu, left)) break;
+              weights(y);
+              product([&](float (&d)[4], const uint32_t (&va)[4], int t) {
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816h(part, va, pb[t][0], pb[t][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[e] = fmaf(part[e], down, d[e]);
+              });
             }
           }
         }
@@ -535,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
       for (int x = 0; x < 2; ++x) {
         merged(8 * t + 2 * c + x, em, dummy);
         f[t][x] = ex2_approx(m[t][x] - (em == -CUDART_INF_F ? 0.f : em));
-        if (I8) f[t][x] *= power_of_2(kv);
+        if (I8) f[t][x] *= power_of_2(kv[t][x]);
       }
     merged(er, em, el);
     const bool split = w.off > 0 || cnt < w.nb;

@@ -484,6 +484,43 @@ def test_attention_int8_rows_of_very_different_scales(n, q_amp, v_lo, v_hi):
     p.check()
 
 
+@pytest.mark.parametrize("n,H,Hk", [(2, 2, 2), (3, 4, 2), (8, 4, 2), (4, 8, 1), (150, 2, 2)])
+def test_attention_int8_later_keys_of_any_scale_stay_masked(n, H, Hk):
+    """The last token's v is 2^60 times the others', or its scales are NaN or infinite: the rows before it do not
+    see it and stay exact, whatever range the last row needs."""
+    for bad in (2.0**60, float("nan"), float("inf")):
+        p = Paged([n], [n + 9], H, Hk, 128, 16, True, seed=33)
+        at = n + 8
+        page, off = int(p.table[0, at // 16]), at % 16
+        p.cache.v_scale[page, :, off] *= bad
+        if bad == bad and bad < math.inf:
+            p.v[0][at] *= bad
+            p.check()
+            continue
+        p.cache.k_scale[page, :, off] *= bad
+        got, lse = p.run()
+        o, a, l = p.exact()
+        got = got.view(n, H, 128)
+        close(got[:n - 1], o[:n - 1], 2.0**-8 * (o.abs() + a)[:n - 1])
+        close(lse[:n - 1], l[:n - 1], 1e-4 + 1e-5 * l.abs()[:n - 1])
+        assert not torch.isfinite(got[n - 1]).any()
+
+
+@pytest.mark.parametrize("n,H,Hk", [(1, 8, 1), (1, 16, 1), (2, 8, 2), (40, 4, 2)])
+def test_attention_int8_query_heads_of_very_different_sizes(n, H, Hk):
+    """Query heads that share a key head, every other one 2^-25 of the rest: with keys of size 2^25 the small
+    ones have ordinary scores and stay exact."""
+    p = Paged([n], [300], H, Hk, 128, 16, True, seed=34)
+    small = torch.arange(H, device="cuda") % 2 == 1
+    p.q.view(n, H, 128)[:, small] *= 2.0**-25
+    p.cache.k_scale *= 2.0**25
+    p.k[0] *= 2.0**25
+    got, lse = p.run()
+    o, a, l = p.exact()
+    close(got.view(n, H, 128)[:, small], o[:, small], 2.0**-8 * (o.abs() + a)[:, small])
+    close(lse[:, small], l[:, small], 1e-4 + 1e-5 * l.abs()[:, small])
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("n,H,Hk", [(3, 2, 2), (4, 8, 1), (150, 2, 2)])
 def test_attention_nonfinite_values_of_later_keys_stay_masked(n, H, Hk, bad):
