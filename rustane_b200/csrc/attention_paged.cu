@@ -19,7 +19,7 @@
 // to bf16 for the P V product (its sum is not): 2^-9 of each weight.
 //
 // Measured, of the copy rate: 8 sequences of up to 40037 tokens, 32 query and 8 key heads, 176 us
-// (99%); 48 x 3000 of 16 heads 203 us (99%); 48 x up to 6011 tokens of 32 heads in int8 255 us (77%:
+// (99%); 48 x 3000 of 16 heads 203 us (99%); 48 x up to 6011 tokens of 32 heads in int8 253 us (78%:
 // the conversion's integer instructions); one sequence of 512 tokens of 12 heads 9.3 us, most of
 // it the launch and a chain of dependent loads (lengths, page, keys) and the join.
 //
@@ -465,19 +465,22 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
             // row's O has fallen, and no further than it fell, so that O's own numbers do not grow.
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
+              auto exponent = [](float w) {  // of a finite weight, else 0
+                const unsigned x = __float_as_uint(w) >> 23 & 0xffu;
+                return x < 255 ? x : 0u;
+              };
+              unsigned top = max(exponent(s[t][0]), exponent(s[t][2])) | max(exponent(s[t][1]), exponent(s[t][3])) << 16;
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
               float f[2];
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
-                const unsigned x0 = __float_as_uint(s[t][x]) & 0x7fffffffu, x1 = __float_as_uint(s[t][2 + x]) & 0x7fffffffu;
-                unsigned top = max(x0 < 0x7f800000u ? x0 : 0u, x1 < 0x7f800000u ? x1 : 0u);
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-                const int above = static_cast<int>(top >> 23) - 127 - kv[t][x];
+                const int ex = top >> 16 * x & 0xffffu, above = ex - 127 - kv[t][x];
                 int to = kv[t][x];
-                if (top && above >= 15) to += above - 10;
-                else if (top && above < 0) to += max(above - 10, -fell[t][x]);
+                if (ex && above >= 15) to += above - 10;
+                else if (ex && above < 0) to += max(above - 10, -fell[t][x]);
                 to = max(max(-100, kv[t][x] - 120), min(120, to));
-                f[x] = ldexpf(1.f, kv[t][x] - to);
+                f[x] = kv[t][x] - to < -126 ? 0.f : power_of_2(kv[t][x] - to);
                 kv[t][x] = to;
               }
 #pragma unroll
