@@ -12,8 +12,8 @@
 // columns, NT times: with the query rows as the 16, a step of 1 to 8 rows issued twice the
 // products and held twice the sums.
 //
-// 160 threads a CTA, three CTAs an SM (NT 2: two): warp 4 streams 64-key blocks by TMA (one box
-// per page and 128 bytes of head, swizzled) into a ring of 64 KB (96 KB); warps 0-3 take 16 keys
+// 160 threads a CTA, three CTAs an SM (NT 2: two; hd 64: one more): warp 4 streams 64-key blocks by TMA (one box
+// per page and 128 bytes of head, swizzled) into a ring of 64 KB (NT 2: 96 KB); warps 0-3 take 16 keys
 // of each block for all rows, each with its own running maximum, sum and output, which meet in
 // the last block's ring slot when the item (or the CTA's part of it) ends.  P is rounded
 // to bf16 for the P V product (its sum is not): 2^-9 of each weight.
@@ -49,8 +49,11 @@ constexpr int kThreads = (kConsumers + 1) * 32;
 template <int HD, bool I8, int NT>
 struct Cfg {
   static constexpr int BM = 8 * NT;                    // rows per tile
-  static constexpr int CTAS = NT == 1 ? 3 : 2;         // an SM
-  static constexpr int RING_BYTES = NT == 1 ? 64 * 1024 : 96 * 1024;
+  // As many CTAs an SM as the registers allow; they share the shared memory.  hd 64, 48 x up to 6011
+  // tokens of 32 heads: four 199 us (int8 193), three 211 (227), five, with spills, 210 (225).  hd 128 in int8
+  // with four: 265 against 252.
+  static constexpr int CTAS = (NT == 1 ? 3 : 2) + (HD == 64 ? 1 : 0);
+  static constexpr int RING_BYTES = (NT == 1 ? (HD == 64 ? 46 : 64) : HD == 64 ? 62 : 96) * 1024;
   static constexpr int ROW = HD * (I8 ? 1 : 2);  // bytes of a key
   static constexpr int TILE = kBK * ROW;
   static constexpr int SCALES = I8 ? kBK * 4 : 0;
