@@ -15,8 +15,9 @@
 // 160 threads a CTA, three CTAs an SM (NT 2: two; hd 64: one more): warp 4 streams 64-key blocks by TMA (one box
 // per page and 128 bytes of head, swizzled) into a ring of 64 KB (NT 2: 96 KB); warps 0-3 take 16 keys
 // of each block for all rows, each with its own running maximum, sum and output, which meet in
-// the last block's ring slot when the item (or the CTA's part of it) ends.  P is rounded
-// to bf16 for the P V product (its sum is not): 2^-9 of each weight.
+// the last block's ring slot when the item (or the CTA's part of it) ends.  A weight goes into the
+// P V product as the sum of two bf16 numbers, 2^-15 of it off: its leading 8 bits, then what they leave
+// (2^-7 of it).  Both are above 0 where the weight is, so that an infinite v stays infinite.
 //
 // Measured, of the copy rate: 8 sequences of up to 40037 tokens, 32 query and 8 key heads, 176 us
 // (99%); 48 x 3000 of 16 heads 203 us (99%); 48 x up to 6011 tokens of 32 heads in int8 253 us (78%:
@@ -45,6 +46,7 @@ namespace {
 constexpr int kBK = 64;   // keys per block
 constexpr int kConsumers = 4;
 constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr float kLeft = 0x1p-18f;  // of a weight, added to what its leading bits leave: never 0
 
 template <int HD, bool I8, int NT>
 struct Cfg {
@@ -424,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
           }
         }
         // ------------------------------------------------------- P^T: 16 keys x 8 NT rows
-        uint32_t pb[NT][2];
+        uint32_t pb[NT][2], pr[NT][2];  // pr (bf16): what pb leaves of the weight
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -439,8 +441,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
             }
           }
           if (!I8) {
-            pb[t][0] = transpose8(pack_bf16x2(s[t][0], s[t][1]));
-            pb[t][1] = transpose8(pack_bf16x2(s[t][2], s[t][3]));
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float z0 = s[t][2 * x], z1 = s[t][2 * x + 1];
+              const uint32_t lead = __byte_perm(__float_as_uint(z0), __float_as_uint(z1), 0x7632);
+              pb[t][x] = transpose8(lead);
+              pr[t][x] = transpose8(pack_bf16x2(fmaf(z0, kLeft, z0 - bf16lo(lead)), fmaf(z1, kLeft, z1 - bf16hi(lead))));
+            }
           }
         }
         float y[NT][4];
@@ -523,7 +530,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
               va[3] &= keep[1];
             }
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma16816(o[dg][t], va, pb[t][0], pb[t][1]);
+            for (int t = 0; t < NT; ++t) {
+              mma16816(o[dg][t], va, pb[t][0], pb[t][1]);
+              mma16816(o[dg][t], va, pr[t][0], pr[t][1]);
+            }
           }
         } else {
           const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);

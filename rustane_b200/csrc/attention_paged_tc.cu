@@ -26,7 +26,8 @@
 // Other forms, same cases: one stream of two threads a row 115; one S buffer of 128 keys a
 // stream 157; S of 128 keys into both buffers 107; P in shared memory 108; exponentials partly on the FMA
 // pipe 104 and up; int8 with a branch for unseen weights inside the exponent loop +13%.
-// P is rounded to bf16 for the P V product (its sum is not).  All waits are bounded.
+// P is rounded to bf16 for the P V product (its sum is not), 2^-8 of each weight, as in the training forward: a
+// product for the remainder would add half as much again to the products of a step.  All waits are bounded.
 #include "attention_paged.cuh"
 #include "kernels.h"
 
