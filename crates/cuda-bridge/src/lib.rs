@@ -246,6 +246,7 @@ extern "C" {
     pub fn rt_kernel_kv_append(qkv: *const c_void, ldqkv: i64, q_out: *mut c_void, ldq: i64, pos: *const i32, slots: *const i32, rope: *const rt_rope, gamma_q: *const f32, gamma_k: *const f32, eps: f32, cache: *const rt_kv_pages, T: c_int, heads: c_int, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
     pub fn rt_kernel_kv_gather(cache: *const rt_kv_pages, slots: *const i32, k_out: *mut c_void, v_out: *mut c_void, ldo: i64, T: c_int, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
     pub fn rt_kernel_attention_paged(q: *const c_void, ldq: i64, out: *mut c_void, ldo: i64, lse2: *mut f32, cache: *const rt_kv_pages, page_table: *const i32, table_ld: i64, kv_lens: *const i32, q_start: *const i32, nseq: c_int, T: c_int, max_q: c_int, max_kv: c_int, heads: c_int, window: c_int, scale: f32, workspace: *mut c_void, workspace_bytes: i64, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
+    pub fn rt_kernel_attention_paged_cols(q: *const c_void, ldq: i64, out: *mut c_void, ldo: i64, lse2: *mut f32, cache: *const rt_kv_pages, page_table: *const i32, table_ld: i64, table_cols: i64, kv_lens: *const i32, q_start: *const i32, nseq: c_int, T: c_int, max_q: c_int, max_kv: c_int, heads: c_int, window: c_int, scale: f32, workspace: *mut c_void, workspace_bytes: i64, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
     pub fn rt_kernel_attention_paged_workspace_bytes(hd: c_int) -> i64;
     pub fn rt_kernel_logits_adjust(logits: *const f32, ldl: i64, out: *mut f32, ldo: i64, token: *mut i32, B: c_int, V: c_int, rules: *const rt_logit_rules, dev_err: *mut c_int, stream: *mut c_void) -> c_int;
 }

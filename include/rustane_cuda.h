@@ -495,6 +495,14 @@ RT_API int rt_kernel_attention_paged(const void* q, int64_t ldq, void* out, int6
                                      const int32_t* kv_lens, const int32_t* q_start, int nseq, int T, int max_q,
                                      int max_kv, int heads, int window, float scale, void* workspace,
                                      int64_t workspace_bytes, int* dev_err, void* stream);
+/* The same for a page table whose rows, table_ld entries apart, hold table_cols entries each (a part of a
+ * wider table; table_ld 0: one row for all sequences).  No other entry is read; a length outside [0,
+ * table_cols * page_size] counts as 0 and sets dev_err. */
+RT_API int rt_kernel_attention_paged_cols(const void* q, int64_t ldq, void* out, int64_t ldo, float* lse2,
+                                          const rt_kv_pages* cache, const int32_t* page_table, int64_t table_ld,
+                                          int64_t table_cols, const int32_t* kv_lens, const int32_t* q_start, int nseq,
+                                          int T, int max_q, int max_kv, int heads, int window, float scale,
+                                          void* workspace, int64_t workspace_bytes, int* dev_err, void* stream);
 RT_API int64_t rt_kernel_attention_paged_workspace_bytes(int hd);
 
 /* What changes a row of logits before a token is chosen; null: not applied.  hist: each

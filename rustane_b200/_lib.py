@@ -166,6 +166,9 @@ SIGNATURES: dict[str, tuple] = {
     "rt_kernel_attention_paged": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, P_KV, c_void_p, c_int64,
                                           c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float,
                                           c_void_p, c_int64, c_void_p, c_void_p]),
+    "rt_kernel_attention_paged_cols": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, P_KV, c_void_p, c_int64,
+                                               c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
+                                               c_float, c_void_p, c_int64, c_void_p, c_void_p]),
     "rt_kernel_attention_paged_workspace_bytes": (c_int64, [c_int]),
     "rt_kernel_logits_adjust": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int,
                                         ctypes.POINTER(RtLogitRules), c_void_p, c_void_p]),

@@ -831,7 +831,7 @@ int64_t attn_paged_workspace_bytes(int hd) {
 int attn_paged(const PagedAttnArgs& a, cudaStream_t s) {
   if (!kv_pages_ok(a.cache) || a.nseq < 0 || a.T < 0 || a.heads <= 0 || a.heads % a.cache.kv_heads) return -1;
   const int64_t cols = static_cast<int64_t>(a.heads) * a.cache.hd;
-  if (a.ldq % 8 || a.ldo % 8 || a.ldq < cols || a.ldo < cols || a.table_ld < 0 || a.window < 0) return -1;
+  if (a.ldq % 8 || a.ldo % 8 || a.ldq < cols || a.ldo < cols || a.table_ld < 0 || a.table_cols < 0 || a.window < 0) return -1;
   if (!(a.scale > 0.f)) return -1;
   if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.workspace)) & 15)
     return -1;
@@ -842,8 +842,8 @@ int attn_paged(const PagedAttnArgs& a, cudaStream_t s) {
   p.a = a;
   p.G = a.heads / a.cache.kv_heads;
   p.page_shift = 31 - __builtin_clz(a.cache.page_size);
-  const int64_t room = a.table_ld * a.cache.page_size;
-  p.max_len = static_cast<int>(room < (1 << 30) ? room : 1 << 30);
+  const int64_t most_pages = (1 << 30) / a.cache.page_size;
+  p.max_len = static_cast<int>((a.table_cols < most_pages ? a.table_cols : most_pages) * a.cache.page_size);
   p.scale_log2 = a.scale * 1.4426950408889634f;
   // Up to 8 or 16 rows per key head and sequence fill one tile of the kernel above; more rows share
   // each block's keys in tiles of up to 2 x 128 on the tcgen05 tensor cores.

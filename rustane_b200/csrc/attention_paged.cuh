@@ -32,7 +32,7 @@ struct Params {
   int bm;          // rows per tile
   int tile_tokens; // bm / G where that is whole, else 0
   int page_shift;
-  int max_len;     // tokens a row of the page table holds
+  int max_len;     // tokens the entries of a row of the page table hold
   float scale_log2;
 };
 

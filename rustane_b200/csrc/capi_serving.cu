@@ -138,11 +138,11 @@ RT_API int rt_kernel_kv_gather(const rt_kv_pages* cache, const int32_t* slots, v
 
 RT_API int64_t rt_kernel_attention_paged_workspace_bytes(int hd) { return rt::attn_paged_workspace_bytes(hd); }
 
-RT_API int rt_kernel_attention_paged(const void* q, int64_t ldq, void* out, int64_t ldo, float* lse2,
-                                     const rt_kv_pages* cache, const int32_t* page_table, int64_t table_ld,
-                                     const int32_t* kv_lens, const int32_t* q_start, int nseq, int T, int max_q,
-                                     int max_kv, int heads, int window, float scale, void* workspace,
-                                     int64_t workspace_bytes, int* dev_err, void* stream) {
+RT_API int rt_kernel_attention_paged_cols(const void* q, int64_t ldq, void* out, int64_t ldo, float* lse2,
+                                          const rt_kv_pages* cache, const int32_t* page_table, int64_t table_ld,
+                                          int64_t table_cols, const int32_t* kv_lens, const int32_t* q_start, int nseq,
+                                          int T, int max_q, int max_kv, int heads, int window, float scale,
+                                          void* workspace, int64_t workspace_bytes, int* dev_err, void* stream) {
   if (!pages_given(cache) || !workspace) return RT_ERR_ARG;
   if (T > 0 && nseq > 0 && (!q || !out || !page_table || !kv_lens || !q_start)) return RT_ERR_ARG;
   rt::PagedAttnArgs a;
@@ -154,6 +154,7 @@ RT_API int rt_kernel_attention_paged(const void* q, int64_t ldq, void* out, int6
   a.cache = pages(cache);
   a.table = page_table;
   a.table_ld = table_ld;
+  a.table_cols = table_cols;
   a.kv_lens = kv_lens;
   a.q_start = q_start;
   a.nseq = nseq;
@@ -167,6 +168,16 @@ RT_API int rt_kernel_attention_paged(const void* q, int64_t ldq, void* out, int6
   a.workspace_bytes = workspace_bytes;
   a.err = dev_err;
   return map_rc(rt::attn_paged(a, st(stream)));
+}
+
+RT_API int rt_kernel_attention_paged(const void* q, int64_t ldq, void* out, int64_t ldo, float* lse2,
+                                     const rt_kv_pages* cache, const int32_t* page_table, int64_t table_ld,
+                                     const int32_t* kv_lens, const int32_t* q_start, int nseq, int T, int max_q,
+                                     int max_kv, int heads, int window, float scale, void* workspace,
+                                     int64_t workspace_bytes, int* dev_err, void* stream) {
+  return rt_kernel_attention_paged_cols(q, ldq, out, ldo, lse2, cache, page_table, table_ld, table_ld, kv_lens, q_start,
+                                        nseq, T, max_q, max_kv, heads, window, scale, workspace, workspace_bytes,
+                                        dev_err, stream);
 }
 
 RT_API int rt_kernel_logits_adjust(const float* logits, int64_t ldl, float* out, int64_t ldo, int32_t* token, int B,

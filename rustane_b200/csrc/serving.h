@@ -71,8 +71,9 @@ struct PagedAttnArgs {
   int64_t ldo = 0;
   float* lse2 = nullptr;  // [T, heads] or null
   KvPages cache;
-  const int32_t* table = nullptr;  // [nseq, table_ld] page numbers
+  const int32_t* table = nullptr;  // [nseq, table_cols] page numbers, rows table_ld apart
   int64_t table_ld = 0;
+  int64_t table_cols = 0;  // entries of a row
   const int32_t* kv_lens = nullptr;  // [nseq]
   const int32_t* q_start = nullptr;  // [nseq + 1]
   int nseq = 0, T = 0, heads = 0;

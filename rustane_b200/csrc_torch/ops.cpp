@@ -197,7 +197,8 @@ std::tuple<Tensor, Opt> attention_paged(const Tensor& q, int64_t cache, int64_t 
   const int64_t n = kv_lens.dim() == 1 ? kv_lens.size(0) : -1;
   vec("kv_lens", kv_lens, n, kI32, dev);
   vec("q_start", q_start, n + 1, kI32, dev);
-  const int64_t ldt = rows("page_table", page_table, page_table.dim() == 2 ? page_table.size(1) : 0, kI32, dev, n);
+  const int64_t pages = page_table.dim() == 2 ? page_table.size(1) : 0;  // of a row; its stride may be another number
+  const int64_t ldt = rows("page_table", page_table, pages, kI32, dev, n);
   on("workspace", workspace_dev, dev);
   auto to_int = [](int64_t v) { return static_cast<int>(std::clamp<int64_t>(v, -1, INT32_MAX)); };
   const c10::cuda::CUDAGuard guard(dev);
@@ -205,10 +206,11 @@ std::tuple<Tensor, Opt> attention_paged(const Tensor& q, int64_t cache, int64_t 
   const int64_t ldo = rows("out", out, cols, kBf16, dev, T);
   Opt lse2;
   if (want_lse) lse2 = at::empty({T, heads}, q.options().dtype(kF32));
-  done(rt_kernel_attention_paged(ptr<void>(q), ldq, ptr<void>(out), ldo, ptr<float>(lse2), c, ptr<int32_t>(page_table), ldt,
-                                 ptr<int32_t>(kv_lens), ptr<int32_t>(q_start), n, T, to_int(max_q), to_int(max_kv), heads,
-                                 to_int(window), static_cast<float>(scale), reinterpret_cast<void*>(workspace),
-                                 workspace_bytes, reinterpret_cast<int*>(err), stream(dev)),
+  done(rt_kernel_attention_paged_cols(ptr<void>(q), ldq, ptr<void>(out), ldo, ptr<float>(lse2), c,
+                                      ptr<int32_t>(page_table), ldt, pages, ptr<int32_t>(kv_lens), ptr<int32_t>(q_start),
+                                      n, T, to_int(max_q), to_int(max_kv), heads, to_int(window),
+                                      static_cast<float>(scale), reinterpret_cast<void*>(workspace), workspace_bytes,
+                                      reinterpret_cast<int*>(err), stream(dev)),
        "rt_kernel_attention_paged");
   return {out, lse2};
 }
