@@ -57,6 +57,13 @@ c10::Device cuda(const Tensor& t) {
   TORCH_CHECK_VALUE(t.is_cuda(), "a CUDA tensor is needed");
   return t.device();
 }
+// The device's error word, where one is given.
+int* error_word(const Opt& t, c10::Device dev) {
+  if (t)
+    TORCH_CHECK_VALUE(t->scalar_type() == kI32 && t->numel() > 0 && t->device() == dev, "err: has to be an int32 tensor on ",
+                      dev, ", got ", t->sizes(), " ", t->scalar_type(), " on ", t->device());
+  return ptr<int>(t);
+}
 void* stream(c10::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 void done(int rc, const char* name) {
   if (rc == RT_OK) return;
@@ -103,7 +110,7 @@ Tensor qk_norm_rope(const Tensor& qkv, const Tensor& positions, int64_t rope, in
   const int64_t ldo = rows("out", out, cols, kBf16, dev, T);
   done(rt_kernel_qk_norm_rope_fwd(ptr<void>(qkv), ld, ptr<void>(out), ldo, ptr<int32_t>(positions),
                                   reinterpret_cast<const rt_rope*>(rope), ptr<float>(gamma_q), ptr<float>(gamma_k),
-                                  static_cast<float>(eps), T, heads, kv_heads, nv, hd, ptr<int>(err), stream(dev)),
+                                  static_cast<float>(eps), T, heads, kv_heads, nv, hd, error_word(err, dev), stream(dev)),
        "rt_kernel_qk_norm_rope_fwd");
   return out;
 }
@@ -138,8 +145,8 @@ std::tuple<Tensor, Opt, Opt> qk_norm_rope_backward(const Tensor& dout, const Opt
   done(rt_kernel_qk_norm_rope_bwd(ptr<void>(dout), ld, gamma_q ? ptr<void>(qkv) : nullptr, ldx, ptr<void>(dqkv), lddx,
                                   ptr<int32_t>(positions), reinterpret_cast<const rt_rope*>(rope), ptr<float>(gamma_q),
                                   ptr<float>(gamma_k), static_cast<float>(eps), ptr<float>(dgq), ptr<float>(dgk),
-                                  gamma_q && dgq_given, ptr<float>(partials), T, heads, kv_heads, nv, hd, ptr<int>(err),
-                                  stream(dev)),
+                                  gamma_q && dgq_given, ptr<float>(partials), T, heads, kv_heads, nv, hd,
+                                  error_word(err, dev), stream(dev)),
        "rt_kernel_qk_norm_rope_bwd");
   return {dqkv, dgq, dgk};
 }
@@ -260,8 +267,8 @@ std::tuple<Tensor, Tensor> logits_adjust(const Tensor& logits, const Opt& hist, 
   const Tensor out = out_given ? *out_given : like(logits);
   const int64_t ldo = rows("out", out, V, kF32, dev, B);
   const Tensor token = at::empty({B}, logits.options().dtype(kI32));
-  done(rt_kernel_logits_adjust(ptr<float>(logits), ldl, ptr<float>(out), ldo, ptr<int32_t>(token), B, V, &r, ptr<int>(err),
-                               stream(dev)),
+  done(rt_kernel_logits_adjust(ptr<float>(logits), ldl, ptr<float>(out), ldo, ptr<int32_t>(token), B, V, &r,
+                               error_word(err, dev), stream(dev)),
        "rt_kernel_logits_adjust");
   return {out, token};
 }
