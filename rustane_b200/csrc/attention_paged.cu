@@ -844,6 +844,7 @@ int attn_paged(const PagedAttnArgs& a, cudaStream_t s) {
   p.page_shift = 31 - __builtin_clz(a.cache.page_size);
   const int64_t most_pages = (1 << 30) / a.cache.page_size;
   p.max_len = static_cast<int>((a.table_cols < most_pages ? a.table_cols : most_pages) * a.cache.page_size);
+  if (a.window >= p.max_len) p.a.window = 0;  // of no length: and differences with it stay in 32 bits
   p.scale_log2 = a.scale * 1.4426950408889634f;
   // Up to 8 or 16 rows per key head and sequence fill one tile of the kernel above; more rows share
   // each block's keys in tiles of up to 2 x 128 on the tcgen05 tensor cores.
