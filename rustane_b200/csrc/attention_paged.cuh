@@ -201,17 +201,20 @@ __device__ __forceinline__ int block_owner(int64_t x, int64_t total, int P) {
   return static_cast<int>(((x + 1) * P - 1) / total);
 }
 
-__device__ __forceinline__ int page_of(const Params& p, const int32_t* table, int key) {
-  const int page = table[key >> p.page_shift];
+__device__ __forceinline__ int checked_page(const Params& p, int page) {
   if (page >= 0 && page < p.a.cache.num_pages) return page;
   set_error(p.a.err, kDevBadIndex);
   return 0;
+}
+__device__ __forceinline__ int page_of(const Params& p, const int32_t* table, int key) {
+  return checked_page(p, table[key >> p.page_shift]);
 }
 
 // Keys [lo, hi) of head h for one row, one warp, fp32 throughout: running maximum m (log2
 // domain), sum l and the lane's HD / 32 entries of the unnormalised output.  Only keys of
 // the range are touched.  The tile kernels weigh keys that a row does not see by 0, which
-// a NaN or infinite v turns into NaN; rows that came out NaN take this instead.
+// a NaN or infinite v turns into NaN; rows that came out NaN take this instead (of the few-row kernel, a
+// warp of which has 4 at most; it needs few registers, which the main loop would miss).
 template <int HD>
 __device__ __noinline__ void row_attend(const Params& p, const int32_t* table, int h, const __nv_bfloat16* qrow, int lo,
                                         int hi, float& m, float& l, float (&o)[HD / 32]) {
