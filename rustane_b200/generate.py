@@ -16,6 +16,7 @@ form (rotation out of place, causal attention without a cache) and returns per-t
 """
 from __future__ import annotations
 
+import functools
 import math
 import sys
 from dataclasses import dataclass, field
@@ -37,6 +38,15 @@ class Sequence:
     """A request: its pages of the cache and the tokens cached so far."""
     pages: list[int] = field(default_factory=list)
     cached: int = 0
+
+
+def _on_device(method):
+    """The library launches on the current device: the generator's, while `method` runs."""
+    @functools.wraps(method)
+    def call(self, *args, **kw):
+        with torch.cuda.device(self.device):
+            return method(self, *args, **kw)
+    return call
 
 
 class Generator:
@@ -127,6 +137,7 @@ class Generator:
             self.uses[p] -= 1
         seq.pages, seq.cached = [], 0
 
+    @_on_device
     def forward(self, tokens: torch.Tensor, seqs: list[Sequence], counts: list[int]) -> torch.Tensor:
         """Append counts[s] >= 1 new tokens to each sequence (`tokens` int32, concatenated) and return the
         logits [sequences, vocab] after each one's last token."""
@@ -157,6 +168,7 @@ class Generator:
 
         return self._logits(self._blocks(tokens, attend)[d_last.long()].contiguous())
 
+    @_on_device
     def prefill(self, prompts: list[list[int]], chunk: int = 512) -> tuple[list[Sequence], torch.Tensor]:
         """Feed prompts, `chunk` tokens of each at a time; (sequences, logits after each prompt)."""
         seqs = [Sequence() for _ in prompts]
@@ -168,6 +180,7 @@ class Generator:
             logits[on] = self.forward(tok, [seqs[i] for i in on], [len(n) for n in new])
         return seqs, logits
 
+    @_on_device
     def fork(self, seq: Sequence) -> Sequence:
         """A second sequence with the same past: full pages are shared, the last one's tokens are read
         back and written again (position 0 rotates by nothing)."""
@@ -187,6 +200,7 @@ class Generator:
                 ops.kv_append(rows, zero, old + new.pages[full] * ps, self.rope, cache, c.heads)
         return new
 
+    @_on_device
     def generate(self, prompts: list[list[int]], max_new: int, chunk: int = 512, answers: int = 1, repetition: float = 1.0,
                  presence: float = 0.0, frequency: float = 0.0, bias: dict[int, float] | None = None,
                  forbid: list[int] | None = None) -> list[list[list[int]]]:
@@ -237,6 +251,7 @@ class Generator:
                 for i in range(len(prompts))]
 
     # ---------------------------------------------------------------- training form
+    @_on_device
     def score(self, tokens: list[int]) -> torch.Tensor:
         """Losses [len - 1] of a text's tokens 1.. given those before, without the cache."""
         c, n = self.cfg, len(tokens)
@@ -329,10 +344,9 @@ def run(a: Args, out=print) -> None:
     rope = dict(scaling="linear", factor=a.rope_linear) if a.rope_linear > 0 else {}
     g = Generator(cfg, weights, capacity=room * len(a.prompts) * a.answers, page_size=a.page_size, max_pos=a.max_pos,
                   cache_dtype=torch.int8 if a.cache == "int8" else torch.bfloat16, device=a.device, softcap=a.softcap, **rope)
-    with torch.cuda.device(g.device):
-        for prompt in g.generate(a.prompts, a.max_new, a.chunk, a.answers, a.repetition, a.presence, a.frequency, a.bias, a.forbid):
-            for answer in prompt:
-                out(",".join(str(t) for t in answer))
+    for prompt in g.generate(a.prompts, a.max_new, a.chunk, a.answers, a.repetition, a.presence, a.frequency, a.bias, a.forbid):
+        for answer in prompt:
+            out(",".join(str(t) for t in answer))
 
 
 def main(argv: list[str] | None = None) -> int:

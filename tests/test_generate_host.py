@@ -1,0 +1,84 @@
+"""What rustane_b200.generate.Generator does on the host, on the CPU: the library's and the operators' calls are replaced by
+functions that record them, and the device by the CPU."""
+from types import SimpleNamespace
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from rustane_b200 import ModelConfig, generate, ops  # noqa: E402
+
+
+class Current:
+    """Stands for torch.cuda.device: which device is current inside."""
+    now = None
+
+    def __init__(self, device):
+        self.device = device
+
+    def __enter__(self):
+        self.before, Current.now = Current.now, self.device
+
+    def __exit__(self, *_):
+        Current.now = self.before
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """(make, calls): make(pages) gives a Generator; calls are (name, current device)."""
+    calls = []
+    Current.now = None
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: calls.append((name, Current.now)) or 0
+
+    monkeypatch.setattr(generate, "lib", lambda: Lib())
+    monkeypatch.setattr(torch.cuda, "device", Current)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: SimpleNamespace(cuda_stream=0))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda d=None: None)
+
+    def append(qkv, pos, slots, rope, cache, heads, *a):
+        calls.append(("kv_append", Current.now))
+        return torch.zeros(qkv.shape[0], heads * 128, dtype=torch.bfloat16)
+
+    monkeypatch.setattr(ops, "kv_append", append)
+    monkeypatch.setattr(ops, "attention_paged", lambda q, *a, **k: (torch.zeros_like(q), None))
+    monkeypatch.setattr(ops, "qk_norm_rope", lambda qkv, *a, **k: qkv)
+
+    def make(pages=8, page_size=16, int8=False):
+        c = ModelConfig.custom(128, 256, 1, 2, seq=64, vocab=64)
+        g = object.__new__(generate.Generator)
+        g.cfg, g.page_size, g.softcap, g.device = c, page_size, 0.0, torch.device("cpu")
+        w = torch.zeros(1, 1)
+        g.embed = g.embed_b = g.gamma_final = w
+        g.layers = [dict(wqkv=w, wo=w, w13=w, w2=w, gamma1=w, gamma2=w) for _ in range(c.nlayers)]
+        g.rope = None
+
+        def cache():
+            shape = (pages, c.kv_heads, page_size, c.hd)
+            x = SimpleNamespace(err=torch.zeros(1, dtype=torch.int32), check=lambda: None,
+                                k=torch.zeros(shape, dtype=torch.int8 if int8 else torch.bfloat16), k_scale=None, v_scale=None)
+            x.v = x.k.clone()
+            if int8:
+                x.k_scale, x.v_scale = torch.zeros(shape[:3]), torch.zeros(shape[:3])
+            return x
+
+        g.caches = [cache() for _ in range(c.nlayers)]
+        g.uses, g.workspace, g.err, g.alpha = [0] * pages, None, torch.zeros(1, dtype=torch.int32), 0.5
+        return g
+
+    return make, calls
+
+
+def test_the_librarys_calls_run_on_the_generators_device(host):
+    """The library launches on the current device: whichever that is outside, it is the generator's inside."""
+    make, calls = host
+    g = make()
+    seq = generate.Sequence()
+    g.forward(torch.zeros(5, dtype=torch.int32), [seq], [5])
+    g.prefill([[1, 2, 3]])
+    g.score([1, 2, 3])
+    assert {n for n, _ in calls} >= {"rt_kernel_gemm", "rt_kernel_rmsnorm_fwd", "rt_kernel_embed_gather", "rt_kernel_attention_fwd"}
+    assert all(d == g.device for _, d in calls)
+    assert Current.now is None
