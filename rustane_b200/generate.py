@@ -133,14 +133,28 @@ class Generator:
         raise RustaneError(_lib.RT_ERR_OOM, "no free page in the cache")
 
     def free(self, seq: Sequence) -> None:
-        for p in seq.pages:
+        self._back_to(seq, 0, 0)
+
+    def _back_to(self, seq: Sequence, pages: int, cached: int) -> None:
+        """Give back what the sequence took since it had this many pages and cached tokens."""
+        for p in seq.pages[pages:]:
             self.uses[p] -= 1
-        seq.pages, seq.cached = [], 0
+        del seq.pages[pages:]
+        seq.cached = cached
 
     @_on_device
     def forward(self, tokens: torch.Tensor, seqs: list[Sequence], counts: list[int]) -> torch.Tensor:
         """Append counts[s] >= 1 new tokens to each sequence (`tokens` int32, concatenated) and return the
-        logits [sequences, vocab] after each one's last token."""
+        logits [sequences, vocab] after each one's last token.  If it raises, the sequences are as before."""
+        before = [(s, len(s.pages), s.cached) for s in seqs]
+        try:
+            return self._forward(tokens, seqs, counts)
+        except BaseException:
+            for s, pages, cached in before:
+                self._back_to(s, pages, cached)
+            raise
+
+    def _forward(self, tokens: torch.Tensor, seqs: list[Sequence], counts: list[int]) -> torch.Tensor:
         c, ps = self.cfg, self.page_size
         pos, slots, lens = [], [], []
         for s, n in zip(seqs, counts):
@@ -173,11 +187,16 @@ class Generator:
         """Feed prompts, `chunk` tokens of each at a time; (sequences, logits after each prompt)."""
         seqs = [Sequence() for _ in prompts]
         logits = torch.empty((len(prompts), self.cfg.vocab), device=self.device)
-        for at in range(0, max(len(p) for p in prompts), chunk):
-            on = [i for i, p in enumerate(prompts) if len(p) > at]
-            new = [prompts[i][at:at + chunk] for i in on]
-            tok = torch.tensor([t for n in new for t in n], dtype=torch.int32, device=self.device)
-            logits[on] = self.forward(tok, [seqs[i] for i in on], [len(n) for n in new])
+        try:
+            for at in range(0, max(len(p) for p in prompts), chunk):
+                on = [i for i, p in enumerate(prompts) if len(p) > at]
+                new = [prompts[i][at:at + chunk] for i in on]
+                tok = torch.tensor([t for n in new for t in n], dtype=torch.int32, device=self.device)
+                logits[on] = self.forward(tok, [seqs[i] for i in on], [len(n) for n in new])
+        except BaseException:
+            for s in seqs:
+                self.free(s)
+            raise
         return seqs, logits
 
     @_on_device
@@ -189,7 +208,9 @@ class Generator:
         new = Sequence(seq.pages[:full], seq.cached)
         for p in new.pages:
             self.uses[p] += 1
-        if rest:
+        if not rest:
+            return new
+        try:
             new.pages.append(self._page())
             old = torch.arange(rest, dtype=torch.int32, device=self.device)
             zero = torch.zeros_like(old)
@@ -198,6 +219,9 @@ class Generator:
                 rows = torch.cat((torch.zeros((rest, c.q_dim), dtype=torch.bfloat16, device=self.device), k.flatten(1),
                                   v.flatten(1)), 1)
                 ops.kv_append(rows, zero, old + new.pages[full] * ps, self.rope, cache, c.heads)
+        except BaseException:
+            self.free(new)
+            raise
         return new
 
     @_on_device
@@ -207,8 +231,16 @@ class Generator:
         """answers greedy answers of max_new tokens to each prompt, as [prompt][answer][token]."""
         if not prompts or any(not p for p in prompts) or max_new < 1 or not 1 <= answers <= self.cfg.vocab:
             raise ValueError("prompts of one token at least, max_new >= 1, answers from 1 to the vocabulary")
+        held, logits = self.prefill(prompts, chunk)
+        try:
+            return self._answer(prompts, held, logits, max_new, answers, repetition, presence, frequency, bias, forbid)
+        finally:
+            for s in held:
+                self.free(s)
+
+    def _answer(self, prompts, held, logits, max_new, answers, repetition, presence, frequency, bias, forbid):
+        """generate() after the prompts, whose sequences are `held`; the forked ones join them there."""
         V, dev = self.cfg.vocab, self.device
-        seqs, logits = self.prefill(prompts, chunk)
         n = len(prompts) * answers
         cap = max(len(p) for p in prompts) + max_new
         hist = torch.full((n, cap), -1, dtype=torch.int32, device=dev)  # -1: not yet written
@@ -232,7 +264,12 @@ class Generator:
             bits[0, forbid] = 0
             words = np.packbits(bits, axis=1, bitorder="little").view(np.int32).copy()
             rules["mask"] = torch.from_numpy(words).to(dev).expand(n, -1).contiguous()
-        seqs = [s if k == 0 else self.fork(s) for s in seqs for k in range(answers)]
+        seqs = []
+        for s in list(held):
+            seqs.append(s)
+            for _ in range(1, answers):
+                seqs.append(self.fork(s))
+                held.append(seqs[-1])
         logits = logits.repeat_interleave(answers, 0)
         rows, at = torch.arange(n, device=dev), torch.tensor(lens, device=dev)
         for step in range(max_new):
@@ -245,8 +282,6 @@ class Generator:
                 logits = self.forward(token, seqs, [1] * n)
         out = hist.cpu().numpy()
         self.check()
-        for s in seqs:
-            self.free(s)
         return [[out[i * answers + k, lens[i * answers]:lens[i * answers] + max_new].tolist() for k in range(answers)]
                 for i in range(len(prompts))]
 

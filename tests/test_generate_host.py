@@ -6,7 +6,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from rustane_b200 import ModelConfig, generate, ops  # noqa: E402
+from rustane_b200 import ModelConfig, RustaneError, generate, ops  # noqa: E402
+from rustane_b200._lib import RT_ERR_OOM  # noqa: E402
 
 
 class Current:
@@ -82,3 +83,46 @@ def test_the_librarys_calls_run_on_the_generators_device(host):
     assert {n for n, _ in calls} >= {"rt_kernel_gemm", "rt_kernel_rmsnorm_fwd", "rt_kernel_embed_gather", "rt_kernel_attention_fwd"}
     assert all(d == g.device for _, d in calls)
     assert Current.now is None
+
+
+def adjust(logits, **k):
+    return logits, torch.zeros(logits.shape[0], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("prompts,max_new,answers", [([[1] * 40], 20, 1), ([[1] * 20, [2] * 40], 1, 1), ([[1] * 33], 1, 2),
+                                                     ([[1] * 17], 2, 4)])
+def test_a_request_that_does_not_fit_leaves_no_page_behind(host, monkeypatch, prompts, max_new, answers):
+    """It runs out while answering, while the second prompt is fed, and while an answer is forked."""
+    make, _ = host
+    monkeypatch.setattr(ops, "logits_adjust", adjust)
+    monkeypatch.setattr(ops, "kv_gather", lambda cache, slots: [torch.zeros(len(slots), 1, 128)] * 2)
+    g = make(pages=3)
+    with pytest.raises(RustaneError) as e:
+        g.generate(prompts, max_new, answers=answers)
+    assert e.value.code == RT_ERR_OOM
+    assert g.uses == [0, 0, 0]
+    assert len(g.generate([[1] * 30], 10)[0][0]) == 10
+
+
+def test_a_reported_error_leaves_no_page_behind(host, monkeypatch):
+    make, _ = host
+    monkeypatch.setattr(ops, "logits_adjust", adjust)
+    g = make()
+    g.err[0] = 4
+    with pytest.raises(RustaneError):
+        g.generate([[1, 2]], 3)
+    assert g.uses == [0] * 8
+
+
+def test_forward_that_fails_leaves_its_sequences_as_they_were(host, monkeypatch):
+    make, _ = host
+    g = make(pages=3)
+    a, b = generate.Sequence(), generate.Sequence()
+    g.forward(torch.zeros(3, dtype=torch.int32), [a, b], [1, 2])
+    with pytest.raises(RustaneError):
+        g.forward(torch.zeros(60, dtype=torch.int32), [a, b], [20, 40])
+    assert (len(a.pages), a.cached, len(b.pages), b.cached) == (1, 1, 1, 2) and sum(g.uses) == 2
+    monkeypatch.setattr(ops, "attention_paged", lambda *x, **k: 1 / 0)
+    with pytest.raises(ZeroDivisionError):
+        g.forward(torch.zeros(21, dtype=torch.int32), [a, b], [20, 1])
+    assert (len(a.pages), a.cached, len(b.pages), b.cached) == (1, 1, 1, 2) and sum(g.uses) == 2
