@@ -116,13 +116,13 @@ class Generator:
         return logits if self.softcap <= 0 else self.softcap * torch.tanh(logits / self.softcap)
 
     def check(self) -> None:
-        """Wait for the calls so far and raise what they reported."""
-        code = int(self.err.item())
-        if code:
-            self.err.zero_()
-            raise RustaneError(_lib.RT_ERR_TOKEN if code == 4 else _lib.RT_ERR_DEVICE, f"device error code {code}")
-        for cache in self.caches:
-            cache.check()
+        """Wait for the calls so far; clear what they reported and raise the first of it."""
+        words = [self.err] + [cache.err for cache in self.caches]
+        codes = [c for c in torch.cat(words).tolist() if c]
+        if codes:
+            for w in words:
+                w.zero_()
+            raise RustaneError(_lib.RT_ERR_TOKEN if codes[0] == 4 else _lib.RT_ERR_DEVICE, f"device error code {codes[0]}")
 
     # ---------------------------------------------------------------------- serving
     def _page(self) -> int:

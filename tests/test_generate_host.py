@@ -7,7 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from rustane_b200 import ModelConfig, RustaneError, generate, ops  # noqa: E402
-from rustane_b200._lib import RT_ERR_OOM  # noqa: E402
+from rustane_b200._lib import RT_ERR_DEVICE, RT_ERR_OOM, RT_ERR_TOKEN  # noqa: E402
 
 
 class Current:
@@ -58,9 +58,10 @@ def host(monkeypatch):
 
         def cache():
             shape = (pages, c.kv_heads, page_size, c.hd)
-            x = SimpleNamespace(err=torch.zeros(1, dtype=torch.int32), check=lambda: None,
+            x = SimpleNamespace(err=torch.zeros(1, dtype=torch.int32), device=torch.device("cpu"),
                                 k=torch.zeros(shape, dtype=torch.int8 if int8 else torch.bfloat16), k_scale=None, v_scale=None)
             x.v = x.k.clone()
+            x.check = lambda: ops.KvCache.check(x)
             if int8:
                 x.k_scale, x.v_scale = torch.zeros(shape[:3]), torch.zeros(shape[:3])
             return x
@@ -126,3 +127,21 @@ def test_forward_that_fails_leaves_its_sequences_as_they_were(host, monkeypatch)
     with pytest.raises(ZeroDivisionError):
         g.forward(torch.zeros(21, dtype=torch.int32), [a, b], [20, 1])
     assert (len(a.pages), a.cached, len(b.pages), b.cached) == (1, 1, 1, 2) and sum(g.uses) == 2
+
+
+def test_check_clears_every_word_that_it_reports(host):
+    """One request's errors are not the next one's."""
+    make, _ = host
+    g = make()
+    for word, code in ((g.err, 4), (g.caches[0].err, 6), (g.caches[1].err, 6)):
+        word[0] = code
+    with pytest.raises(RustaneError) as e:
+        g.check()
+    assert e.value.code == RT_ERR_TOKEN
+    assert not any(int(w) for w in (g.err, g.caches[0].err, g.caches[1].err))
+    g.check()
+    g.caches[1].err[0] = 6
+    with pytest.raises(RustaneError) as e:
+        g.check()
+    assert e.value.code == RT_ERR_DEVICE
+    g.check()

@@ -20,3 +20,13 @@ def test_a_request_that_does_not_fit_changes_nothing_for_the_next(model):  # noq
             g.generate(**big)
         assert all(n == 0 for n in g.uses)
     assert g.generate(prompts, max_new=9, answers=2) == exp
+
+
+def test_a_request_past_the_rotary_tables_is_reported_once(model):  # noqa: F811
+    cfg, w, tok, _, _ = model
+    g = generate.Generator(cfg, w, capacity=400, max_pos=64)
+    prompt = tok[0, :30].tolist()
+    exp = g.generate([prompt], max_new=5)
+    with pytest.raises(RustaneError):
+        g.generate([tok[1, :80].tolist()], max_new=3)  # every layer's cache reports it
+    assert g.generate([prompt], max_new=5) == exp
