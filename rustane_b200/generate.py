@@ -49,6 +49,14 @@ def _on_device(method):
     return call
 
 
+def _best(logits: torch.Tensor, n: int) -> torch.Tensor:
+    """The n best tokens of each row by the greedy token's rule: equal values by index, never NaN or -inf."""
+    values, tokens = logits.nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf).sort(dim=1, descending=True, stable=True)
+    if not (values[:, :n] > -math.inf).all():
+        raise ValueError(f"fewer than {n} tokens may start an answer")
+    return tokens[:, :n]
+
+
 class Generator:
     """A model's weights on one GPU and a paged cache for `capacity` tokens of all requests together."""
 
@@ -228,7 +236,8 @@ class Generator:
     def generate(self, prompts: list[list[int]], max_new: int, chunk: int = 512, answers: int = 1, repetition: float = 1.0,
                  presence: float = 0.0, frequency: float = 0.0, bias: dict[int, float] | None = None,
                  forbid: list[int] | None = None) -> list[list[list[int]]]:
-        """answers greedy answers of max_new tokens to each prompt, as [prompt][answer][token]."""
+        """answers greedy answers of max_new tokens to each prompt, as [prompt][answer][token].  ValueError where
+        more answers are asked for than there are tokens to start one with."""
         if not prompts or any(not p for p in prompts) or max_new < 1 or not 1 <= answers <= self.cfg.vocab:
             raise ValueError("prompts of one token at least, max_new >= 1, answers from 1 to the vocabulary")
         held, logits = self.prefill(prompts, chunk)
@@ -275,8 +284,7 @@ class Generator:
         for step in range(max_new):
             logits, token = ops.logits_adjust(logits, err=self.err, **rules)
             if step == 0 and answers > 1:  # answer k of a prompt starts with the k-th best token
-                best = logits[::answers].topk(answers, 1).indices
-                token = best.reshape(-1).to(torch.int32)
+                token = _best(logits[::answers], answers).reshape(-1).to(torch.int32)
             hist[rows, at + step] = token
             if step + 1 < max_new:
                 logits = self.forward(token, seqs, [1] * n)

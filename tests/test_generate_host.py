@@ -145,3 +145,37 @@ def test_check_clears_every_word_that_it_reports(host):
         g.check()
     assert e.value.code == RT_ERR_DEVICE
     g.check()
+
+
+NAN, INF = float("nan"), float("inf")
+
+
+@pytest.mark.parametrize("row,answers,exp", [([1, 3, 2, 3], 3, [1, 3, 2]),          # equal values: the lower index first
+                                             ([NAN, 1, NAN, 2], 2, [3, 1]),         # NaN is never chosen
+                                             ([0, INF, -5, -INF], 3, [1, 0, 2])])
+def test_first_tokens_of_several_answers(host, monkeypatch, row, answers, exp):
+    """The best ones by the greedy token's own rule."""
+    make, _ = host
+    g = make(pages=40)
+    logits = torch.full((1, 64), -INF)
+    logits[0, :4] = torch.tensor(row)
+    monkeypatch.setattr(g, "_logits", lambda x: logits.expand(x.shape[0], -1).clone())
+    monkeypatch.setattr(ops, "logits_adjust", adjust)
+    monkeypatch.setattr(ops, "kv_gather", lambda cache, slots: [torch.zeros(len(slots), 1, 128)] * 2)
+    out = g.generate([[1, 2], [3]], 2, answers=answers)
+    assert [[a[0] for a in p] for p in out] == [exp, exp]
+
+
+@pytest.mark.parametrize("max_new", [1, 3])
+def test_fewer_tokens_than_answers_are_refused(host, monkeypatch, max_new):
+    make, _ = host
+    g = make(pages=40)
+    logits = torch.full((1, 64), -INF)
+    logits[0, :3] = torch.tensor([1, 2, NAN])
+    monkeypatch.setattr(g, "_logits", lambda x: logits.expand(x.shape[0], -1).clone())
+    monkeypatch.setattr(ops, "logits_adjust", adjust)
+    monkeypatch.setattr(ops, "kv_gather", lambda cache, slots: [torch.zeros(len(slots), 1, 128)] * 2)
+    assert [a[0] for a in g.generate([[1]], max_new, answers=2)[0]] == [1, 0]
+    with pytest.raises(ValueError, match="answer"):
+        g.generate([[1]], max_new, answers=3)
+    assert not any(g.uses)

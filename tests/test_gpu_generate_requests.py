@@ -30,3 +30,16 @@ def test_a_request_past_the_rotary_tables_is_reported_once(model):  # noqa: F811
     with pytest.raises(RustaneError):
         g.generate([tok[1, :80].tolist()], max_new=3)  # every layer's cache reports it
     assert g.generate([prompt], max_new=5) == exp
+
+
+def test_forbidden_tokens_start_no_answer(model):  # noqa: F811
+    cfg, w, tok, _, _ = model
+    g = generate.Generator(cfg, w, capacity=400, max_pos=256)
+    p = [tok[0, :9].tolist(), tok[1, :21].tolist()]
+    out = g.generate(p, max_new=3, answers=3, forbid=[t for t in range(cfg.vocab) if t not in (5, 17, 900, 1000)])
+    for answers in out:
+        firsts = [a[0] for a in answers]
+        assert len(set(firsts)) == 3 and all(t in (5, 17, 900, 1000) for a in answers for t in a)
+    with pytest.raises(ValueError):
+        g.generate(p, max_new=3, answers=3, forbid=[t for t in range(cfg.vocab) if t not in (5, 900)])
+    assert not any(g.uses)
