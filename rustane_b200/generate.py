@@ -209,10 +209,8 @@ class Generator:
 
     @_on_device
     def fork(self, seq: Sequence) -> Sequence:
-        """A second sequence with the same past: full pages are shared, the last one's tokens are read
-        back and written again (position 0 rotates by nothing)."""
-        ps, c = self.page_size, self.cfg
-        full, rest = divmod(seq.cached, ps)
+        """A second sequence with the same past: full pages are shared, the last one is copied as it is."""
+        full, rest = divmod(seq.cached, self.page_size)
         new = Sequence(seq.pages[:full], seq.cached)
         for p in new.pages:
             self.uses[p] += 1
@@ -220,13 +218,10 @@ class Generator:
             return new
         try:
             new.pages.append(self._page())
-            old = torch.arange(rest, dtype=torch.int32, device=self.device)
-            zero = torch.zeros_like(old)
-            for cache in self.caches:
-                k, v = ops.kv_gather(cache, old + seq.pages[full] * ps)
-                rows = torch.cat((torch.zeros((rest, c.q_dim), dtype=torch.bfloat16, device=self.device), k.flatten(1),
-                                  v.flatten(1)), 1)
-                ops.kv_append(rows, zero, old + new.pages[full] * ps, self.rope, cache, c.heads)
+            for c in self.caches:
+                for t in (c.k, c.v, c.k_scale, c.v_scale):
+                    if t is not None:
+                        t[new.pages[full]].copy_(t[seq.pages[full]])
         except BaseException:
             self.free(new)
             raise

@@ -96,7 +96,6 @@ def test_a_request_that_does_not_fit_leaves_no_page_behind(host, monkeypatch, pr
     """It runs out while answering, while the second prompt is fed, and while an answer is forked."""
     make, _ = host
     monkeypatch.setattr(ops, "logits_adjust", adjust)
-    monkeypatch.setattr(ops, "kv_gather", lambda cache, slots: [torch.zeros(len(slots), 1, 128)] * 2)
     g = make(pages=3)
     with pytest.raises(RustaneError) as e:
         g.generate(prompts, max_new, answers=answers)
@@ -161,7 +160,6 @@ def test_first_tokens_of_several_answers(host, monkeypatch, row, answers, exp):
     logits[0, :4] = torch.tensor(row)
     monkeypatch.setattr(g, "_logits", lambda x: logits.expand(x.shape[0], -1).clone())
     monkeypatch.setattr(ops, "logits_adjust", adjust)
-    monkeypatch.setattr(ops, "kv_gather", lambda cache, slots: [torch.zeros(len(slots), 1, 128)] * 2)
     out = g.generate([[1, 2], [3]], 2, answers=answers)
     assert [[a[0] for a in p] for p in out] == [exp, exp]
 
@@ -174,7 +172,6 @@ def test_fewer_tokens_than_answers_are_refused(host, monkeypatch, max_new):
     logits[0, :3] = torch.tensor([1, 2, NAN])
     monkeypatch.setattr(g, "_logits", lambda x: logits.expand(x.shape[0], -1).clone())
     monkeypatch.setattr(ops, "logits_adjust", adjust)
-    monkeypatch.setattr(ops, "kv_gather", lambda cache, slots: [torch.zeros(len(slots), 1, 128)] * 2)
     assert [a[0] for a in g.generate([[1]], max_new, answers=2)[0]] == [1, 0]
     with pytest.raises(ValueError, match="answer"):
         g.generate([[1]], max_new, answers=3)

@@ -43,3 +43,27 @@ def test_forbidden_tokens_start_no_answer(model):  # noqa: F811
     with pytest.raises(ValueError):
         g.generate(p, max_new=3, answers=3, forbid=[t for t in range(cfg.vocab) if t not in (5, 900)])
     assert not any(g.uses)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.int8])
+def test_a_forked_sequence_has_the_same_past(model, dtype):  # noqa: F811
+    """Bit for bit, codes and scales, also of an infinite key; and what follows does not touch the source."""
+    cfg, w, tok, _, _ = model
+    g = generate.Generator(cfg, w, capacity=200, cache_dtype=dtype, max_pos=256)
+    (seq,), _ = g.prefill([tok[0, :37].tolist()])
+    if dtype == torch.bfloat16:
+        g.caches[0].k[seq.pages[2], :, 3, 8] = float("inf")
+    new = g.fork(seq)
+    assert new.pages[:2] == seq.pages[:2] and new.pages[2] != seq.pages[2] and new.cached == 37
+
+    def rows(s):  # the last page's 5 tokens
+        return [t[s.pages[2], :, :5] for c in g.caches for t in (c.k, c.v, c.k_scale, c.v_scale) if t is not None]
+
+    before = [r.clone() for r in rows(seq)]
+    assert all(torch.equal(a, b) for a, b in zip(rows(new), before))
+    g.forward(torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda"), [new], [3])
+    assert all(torch.equal(a, b) for a, b in zip(rows(seq), before))
+    assert all(torch.equal(a, b) for a, b in zip(rows(new), before))
+    g.free(seq)
+    g.free(new)
+    assert not any(g.uses)
