@@ -293,9 +293,11 @@ class Generator:
     def score(self, tokens: list[int]) -> torch.Tensor:
         """Losses [len - 1] of a text's tokens 1.. given those before, without the cache."""
         c, n = self.cfg, len(tokens)
+        if n < 2:
+            return torch.empty(0, device=self.device)
         S = -(-n // 128) * 128
         tok = torch.tensor(tokens + [0] * (S - n), dtype=torch.int32, device=self.device)
-        pos = torch.arange(S, dtype=torch.int32, device=self.device)
+        pos = torch.arange(S, dtype=torch.int32, device=self.device).clamp_(max=n - 1)  # the padding takes none of its own
 
         def attend(i: int, qkv: torch.Tensor) -> torch.Tensor:
             qkv = ops.qk_norm_rope(qkv, pos, self.rope, c.heads, c.kv_heads, err=self.err)

@@ -176,3 +176,22 @@ def test_fewer_tokens_than_answers_are_refused(host, monkeypatch, max_new):
     with pytest.raises(ValueError, match="answer"):
         g.generate([[1]], max_new, answers=3)
     assert not any(g.uses)
+
+
+@pytest.mark.parametrize("n", [0, 1])
+def test_score_of_a_text_without_a_second_token_is_empty(host, n):
+    make, calls = host
+    assert make().score([5] * n).shape == (0,)
+    assert not calls
+
+
+@pytest.mark.parametrize("n", [2, 77, 128, 290])
+def test_score_uses_no_position_past_its_text(host, monkeypatch, n):
+    """Whatever the training form's attention pads a text to."""
+    make, _ = host
+    seen = []
+    monkeypatch.setattr(ops, "qk_norm_rope", lambda qkv, pos, *a, **k: seen.append(pos) or qkv)
+    assert make().score([5] * n).shape == (n - 1,)
+    assert len(seen) == 2
+    for pos in seen:
+        assert torch.equal(pos[:n], torch.arange(n, dtype=torch.int32)) and int(pos.max()) == n - 1 and int(pos.min()) == 0

@@ -67,3 +67,14 @@ def test_a_forked_sequence_has_the_same_past(model, dtype):  # noqa: F811
     g.free(seq)
     g.free(new)
     assert not any(g.uses)
+
+
+def test_score_of_a_text_that_just_fits_the_rotary_tables(model):  # noqa: F811
+    cfg, w, tok, _, _ = model
+    text = tok[0, :150].tolist()
+    exp = generate.Generator(cfg, w, capacity=64, max_pos=256).score(text)
+    g = generate.Generator(cfg, w, capacity=64, max_pos=150)
+    assert torch.equal(g.score(text), exp)
+    assert g.score(text[:1]).shape == (0,)
+    with pytest.raises(RustaneError):
+        g.score(text + [1])
