@@ -124,7 +124,8 @@ class Generator:
         return logits if self.softcap <= 0 else self.softcap * torch.tanh(logits / self.softcap)
 
     def check(self) -> None:
-        """Wait for the calls so far; clear what they reported and raise the first of it."""
+        """Wait for the calls so far, of every stream; clear what they reported and raise the first of it."""
+        torch.cuda.synchronize(self.device)
         words = [self.err] + [cache.err for cache in self.caches]
         codes = [c for c in torch.cat(words).tolist() if c]
         if codes:

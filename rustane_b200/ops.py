@@ -118,7 +118,8 @@ class KvCache:
         return cls(k, v, *scales)
 
     def check(self) -> None:
-        """Wait for the error word of the calls so far; raise and clear it if one is set."""
+        """Wait for the calls so far, of every stream; clear the error word and raise if it is set."""
+        torch.cuda.synchronize(self.device)
         code = int(self.err.item())
         if code:
             self.err.zero_()
