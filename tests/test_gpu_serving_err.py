@@ -25,9 +25,12 @@ def test_check_waits_for_calls_of_other_streams():
     _, qkv, pos, rope, _, _ = rope_case(4, 2, 2, 64, 64, "half", False, seed=0)
     cache = ops.KvCache.empty(2, 16, 2, 64, torch.bfloat16, "cuda")
     slots = torch.tensor([0, 1, 32, 2], dtype=torch.int32, device="cuda")
-    torch.cuda.synchronize()
+    good = torch.arange(4, dtype=torch.int32, device="cuda")
     side = torch.cuda.Stream()
+    torch.cuda.synchronize()
     with torch.cuda.stream(side):
+        ops.kv_append(qkv, pos, good, rope, cache, 2)  # the stream's first call loads and allocates, which waits
+        side.synchronize()
         torch.cuda._sleep(100_000_000)  # some 50 ms
         ops.kv_append(qkv, pos, slots, rope, cache, 2)
     with pytest.raises(RustaneError):
