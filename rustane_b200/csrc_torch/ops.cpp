@@ -37,7 +37,7 @@ int64_t rows(const char* name, const Tensor& t, int64_t cols, at::ScalarType typ
                     t.sizes(), " ", t.scalar_type());
   TORCH_CHECK_VALUE(t.device() == dev && (t.size(0) == 0 || t.stride(1) == 1), name,
                     ": its rows have to be contiguous and on ", dev);
-  return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), cols);
+  return t.size(0) > 1 ? t.stride(0) : cols;
 }
 void vec(const char* name, const Tensor& t, int64_t n, at::ScalarType type, c10::Device dev) {
   TORCH_CHECK_VALUE(t.dim() == 1 && t.scalar_type() == type && (n < 0 || t.size(0) == n), name, ": expected ",
