@@ -236,6 +236,8 @@ class Generator:
         more answers are asked for than there are tokens to start one with."""
         if not prompts or any(not p for p in prompts) or max_new < 1 or not 1 <= answers <= self.cfg.vocab:
             raise ValueError("prompts of one token at least, max_new >= 1, answers from 1 to the vocabulary")
+        if any(not 0 <= t < self.cfg.vocab for t in [*(forbid or []), *(bias or {})]):
+            raise ValueError(f"bias and forbid take ids from 0 to {self.cfg.vocab - 1}")
         held, logits = self.prefill(prompts, chunk)
         try:
             return self._answer(prompts, held, logits, max_new, answers, repetition, presence, frequency, bias, forbid)

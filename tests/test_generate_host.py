@@ -195,3 +195,13 @@ def test_score_uses_no_position_past_its_text(host, monkeypatch, n):
     assert len(seen) == 2
     for pos in seen:
         assert torch.equal(pos[:n], torch.arange(n, dtype=torch.int32)) and int(pos.max()) == n - 1 and int(pos.min()) == 0
+
+
+@pytest.mark.parametrize("rules", [dict(forbid=[-1]), dict(forbid=[3, 64]), dict(bias={-1: 2.0}), dict(bias={64: 2.0})])
+def test_rules_for_ids_outside_the_vocabulary_are_refused(host, monkeypatch, rules):
+    """(-1 forbade the vocabulary's last token.)"""
+    make, calls = host
+    monkeypatch.setattr(ops, "logits_adjust", adjust)
+    with pytest.raises(ValueError, match="ids"):
+        make().generate([[1]], 2, **rules)
+    assert not calls
