@@ -5,7 +5,7 @@ Every `.cu` / `.cpp` file under ``rustane_b200/csrc`` is compiled by nvcc for
 ``rustane_b200/librustane_cuda.so`` with the static CUDA runtime.  Objects are
 cached under ``rustane_b200/_build`` and rebuilt when a source or header is
 newer.  ``rustane_b200/csrc_torch/ops.cpp`` (the torch binding of the serving
-operators) is compiled by the host compiler against the installed torch into
+operators) is compiled by the host compiler against the installed torch, where there is one, into
 ``rustane_b200/_torch_ops<suffix>.so``.  No GPU is needed to build.
 """
 from __future__ import annotations
@@ -58,12 +58,14 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
-def build_torch_ext(verbose: bool = False) -> Path:
-    """The torch binding; links librustane_cuda.so (found next to it at run time)."""
-    newest = max([TORCH_SRC.stat().st_mtime] + [h.stat().st_mtime for h in INCLUDE.glob("*.h")])
-    if TORCH_EXT.exists() and TORCH_EXT.stat().st_mtime >= newest:
-        return TORCH_EXT
-    import torch
+def build_torch_ext(verbose: bool = False) -> Path | None:
+    """The torch binding; links librustane_cuda.so (found next to it at run time).  None without torch: the
+    C library does not need it.  Built again when its sources, torch or the command are others than before."""
+    try:
+        import torch
+    except ImportError:
+        print(f"torch is not installed: {TORCH_EXT.name} (rustane_b200.ops) is not built")
+        return None
     root = Path(torch.__file__).parent
     cuda = Path(nvcc()).resolve().parent.parent / "include"
     inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda, INCLUDE,
@@ -72,11 +74,16 @@ def build_torch_ext(verbose: bool = False) -> Path:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_torch_ops",
            *(f"-isystem{i}" for i in inc), str(TORCH_SRC), "-o", str(TORCH_EXT), f"-L{PKG}", "-l:librustane_cuda.so",
            f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    newest = max([TORCH_SRC.stat().st_mtime] + [h.stat().st_mtime for h in INCLUDE.glob("*.h")])
+    made_by, how = BUILD / "torch_ops.txt", f"torch {torch.__version__}\n{' '.join(cmd)}\n"
+    if TORCH_EXT.exists() and TORCH_EXT.stat().st_mtime >= newest and made_by.exists() and made_by.read_text() == how:
+        return TORCH_EXT
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed for {TORCH_SRC.name}:\n{res.stdout}\n{res.stderr}")
+    made_by.write_text(how)
     return TORCH_EXT
 
 
