@@ -393,8 +393,12 @@ def run(a: Args, out=print) -> None:
 
 
 def main(argv: list[str] | None = None) -> int:
+    argv = sys.argv[1:] if argv is None else argv
+    if "--help" in argv or "-h" in argv:
+        print(__doc__)
+        return 0
     try:
-        a = parse_args(sys.argv[1:] if argv is None else argv)
+        a = parse_args(argv)
     except UsageError as e:
         print(e, file=sys.stderr)
         return 1
