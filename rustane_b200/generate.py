@@ -373,6 +373,8 @@ def parse_args(argv: list[str]) -> Args:
         raise UsageError(f"token ids of {a.model} are 0 to {cfg.vocab - 1}")
     if a.cache not in ("bf16", "int8"):
         raise UsageError("--cache: bf16 or int8")
+    if a.page_size not in (16, 32, 64, 128):
+        raise UsageError("--page-size: 16, 32, 64 or 128")
     if a.max_new < 1 or a.chunk < 1 or not 1 <= a.answers <= cfg.vocab:
         raise UsageError("--max-new, --chunk and --answers are 1 at least")
     if max(len(p) for p in a.prompts) + a.max_new > a.max_pos:
