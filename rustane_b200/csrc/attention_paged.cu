@@ -129,7 +129,7 @@ __device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, 128;"
 template <int HD, bool I8, int NT>
 __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
     attn_paged_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                          const __grid_constant__ Params p, int min_blocks) {
+                          const __grid_constant__ Params p) {
   using C = Cfg<HD, I8, NT>;
   constexpr int kBM = C::BM;
   extern __shared__ uint8_t smem_raw[];
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, I8, NT>::CTAS)
   }
   int64_t total;
   int P;
-  Walk<kBK> w = start_walk<kBK, kThreads>(p, min_blocks, total, P);  // its barriers cover the init above
+  Walk<kBK> w = start_walk<kBK, kThreads>(p, total, P);  // its barriers cover the init above
 
   if (warp == kConsumers) {
     // ------------------------------------------------------------------ producer
@@ -806,7 +806,7 @@ int launch(const Params& p, cudaStream_t s) {
   const int64_t keys = p.a.max_kv < 1 ? 1 : p.a.max_kv;
   const int64_t most = p.a.nseq * static_cast<int64_t>(p.a.cache.kv_heads) * tiles * ((keys + kBK - 1) / kBK);
   const int64_t ctas = few_ctas(C::CTAS);
-  attn_paged_few_kernel<HD, I8, NT><<<static_cast<unsigned>(most < ctas ? most : ctas), kThreads, C::BYTES, s>>>(tk, tv, p, 1);
+  attn_paged_few_kernel<HD, I8, NT><<<static_cast<unsigned>(most < ctas ? most : ctas), kThreads, C::BYTES, s>>>(tk, tv, p);
   return cudaGetLastError();
 }
 

@@ -115,7 +115,7 @@ struct Walk {
 // All NT threads of the CTA: the CTA's range of all blocks and its first item.  `total` and
 // `P` (CTAs that share the work) are the same in every CTA.
 template <int BK, int NT>
-__device__ __forceinline__ Walk<BK> start_walk(const Params& p, int min_blocks, int64_t& total, int& P) {
+__device__ __forceinline__ Walk<BK> start_walk(const Params& p, int64_t& total, int& P) {
   __shared__ int64_t warp_sum[NT / 32];
   __shared__ int64_t first_rem, first_head;  // of the CTA's first block in its sequence; the sequence's blocks a head
   __shared__ int first_seq;
@@ -146,8 +146,7 @@ __device__ __forceinline__ Walk<BK> start_walk(const Params& p, int min_blocks, 
     if (i < warp) before += warp_sum[i];
     total += warp_sum[i];
   }
-  const int64_t most = (total + min_blocks - 1) / min_blocks;
-  P = most < gridDim.x ? static_cast<int>(most) : static_cast<int>(gridDim.x);
+  P = total < gridDim.x ? static_cast<int>(total) : static_cast<int>(gridDim.x);
   const int c = blockIdx.x;
   w.g = w.g1 = 0;
   if (c < P) {

@@ -231,7 +231,7 @@ struct Share {
 template <int HD, bool I8>
 __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
     attn_paged_many_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                           const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Params p, int min_blocks) {
+                           const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Params p) {
   using C = Cfg<HD, I8>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(Cfg<HD, I8>::THREADS, 1)
   tc_fence_before();
   int64_t total;
   int P;
-  Walk<kBK> w = start_walk<kBK, C::THREADS>(p, min_blocks, total, P);  // its barriers cover the set-up above
+  Walk<kBK> w = start_walk<kBK, C::THREADS>(p, total, P);  // its barriers cover the set-up above
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // columns [0,128) S0, [128,256) S1, then O0, O1 of 128 each
   auto wait_all = [&](uint64_t* b, uint32_t parity) {  // a whole warp; false: timed out or given up
@@ -964,7 +964,7 @@ int launch(const Params& p, cudaStream_t s) {
   const int64_t most = a.nseq * static_cast<int64_t>(a.cache.kv_heads) * tiles * ((keys + kBK - 1) / kBK);
   const int64_t ctas = attn_paged_many_ctas();
   attn_paged_many_kernel<HD, I8>
-      <<<static_cast<unsigned>(most < ctas ? most : ctas), C::THREADS, C::BYTES, s>>>(tq, tk, tv, p, 1);
+      <<<static_cast<unsigned>(most < ctas ? most : ctas), C::THREADS, C::BYTES, s>>>(tq, tk, tv, p);
   return cudaGetLastError();
 }
 
