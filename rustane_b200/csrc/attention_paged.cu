@@ -13,7 +13,7 @@
 // products and held twice the sums.
 //
 // 160 threads a CTA, three CTAs an SM (NT 2: two; hd 64: one more): warp 4 streams 64-key blocks by TMA (one box
-// per page and 128 bytes of head, swizzled) into a ring of 64 KB (NT 2: 96 KB); warps 0-3 take 16 keys
+// per page and 128 bytes of head, swizzled) into a ring of 32 to 96 KB (Cfg::STAGES blocks); warps 0-3 take 16 keys
 // of each block for all rows, each with its own running maximum, sum and output, which meet in
 // the last block's ring slot when the item (or the CTA's part of it) ends.  A weight goes into the
 // P V product as the sum of two bf16 numbers, 2^-15 of it off: its leading 8 bits, then what they leave
@@ -55,13 +55,14 @@ struct Cfg {
   // tokens of 32 heads: four 199 us (int8 193), three 211 (227), five, with spills, 210 (225).  hd 128 in int8
   // with four: 265 against 252.
   static constexpr int CTAS = (NT == 1 ? 3 : 2) + (HD == 64 ? 1 : 0);
-  static constexpr int RING_BYTES = (NT == 1 ? (HD == 64 ? 46 : 64) : HD == 64 ? 62 : 96) * 1024;
   static constexpr int ROW = HD * (I8 ? 1 : 2);  // bytes of a key
   static constexpr int TILE = kBK * ROW;
   static constexpr int SCALES = I8 ? kBK * 4 : 0;
   static constexpr int STAGE = 2 * TILE + 2 * SCALES;  // K, V, scales of k, of v
   static constexpr int SLOT = (STAGE + 1023) / 1024 * 1024;
-  static constexpr int STAGES = RING_BYTES / SLOT < 8 ? RING_BYTES / SLOT : 8;
+  // Blocks in flight.  hd 64 in bf16 would have the shared memory for one more; 48 x 6011 tokens of 32 heads
+  // take 348 us with two, 361 with three.
+  static constexpr int STAGES = HD == 128 ? (NT == 1 ? (I8 ? 3 : 2) : I8 ? 5 : 3) : NT == 1 ? (I8 ? 5 : 2) : I8 ? 6 : 3;
   static constexpr int BOX = ROW < 128 ? ROW : 128;  // bytes of a row in one TMA box
   static constexpr int BOXES = ROW / BOX;
   // the four warps' outputs meet CHUNK columns at a time in the last block's slot
