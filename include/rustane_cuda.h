@@ -486,7 +486,7 @@ RT_API int rt_kernel_kv_gather(const rt_kv_pages* cache, const int32_t* slots, v
  * and the work follows the device lengths.  A length outside [0, table_ld * page_size]
  * counts as 0 and sets dev_err, a page outside the cache is read as page 0 and sets it.
  * Sums are fp32; for the product with v a weight keeps 15 bits (bf16 cache) or 11 (int8) where max_q * heads /
- * kv_heads is up to 16, and 8 (bf16) where it is more.
+ * kv_heads is up to 16 (or heads / kv_heads is over 128), and 8 (bf16) where it is more.
  * workspace: 16-byte aligned, rt_kernel_attention_paged_workspace_bytes(cache->hd) bytes, zeroed before
  * its first use (and again after a bounded wait ran out); calls that share it run on one
  * stream. */

@@ -20,9 +20,10 @@
 // (2^-7 of it).  Both are above 0 where the weight is, so that an infinite v stays infinite.
 //
 // Measured, of the copy rate: 8 sequences of up to 40037 tokens, 32 query and 8 key heads, 176 us
-// (99%); 48 x 3000 of 16 heads 203 us (99%); 48 x up to 6011 tokens of 32 heads in int8 253 us (78%:
-// the conversion's integer instructions); one sequence of 512 tokens of 12 heads 9.3 us, most of
-// it the launch and a chain of dependent loads (lengths, page, keys) and the join.
+// (99%); 48 x 3000 of 16 heads 183 us (98%); 48 x up to 6011 tokens of 32 heads in int8 253 us (78%); the same
+// at hd 64 191 us (100%), in int8 187 us (54%); one sequence of 512 tokens of 12 heads 9.7 us, most of
+// it the launch and a chain of dependent loads (lengths, page, keys) and the join.  int8 takes two thirds
+// as long at half the head: the rest is work per 16 keys (the maximum across lanes, votes, units, scales).
 //
 // int8: the codes become fp16, exactly (two and a half instructions a pair, one and a half of
 // them on the integer pipe; bf16 takes four and three, and that pipe was the limit: 354 us
@@ -848,7 +849,12 @@ int attn_paged(const PagedAttnArgs& a, cudaStream_t s) {
   if (a.window >= p.max_len) p.a.window = 0;  // of no length: and differences with it stay in 32 bits
   p.scale_log2 = a.scale * 1.4426950408889634f;
   // Up to 8 or 16 rows per key head and sequence fill one tile of the kernel above; more rows share
-  // each block's keys in tiles of up to 2 x 128 on the tcgen05 tensor cores.
+  // each block's keys in tiles of up to 2 x 128 on the tcgen05 tensor cores.  Both kernels, us (few / many), 8
+  // sequences of 8 heads, hd 128 in bf16: 16 rows over 256 keys 12.5 / 15.7, over 2048 28 / 34, over 16384 96 /
+  // 175; 32 rows 12.6 / 15.7, 34 / 35, 171 / 176; 64 rows 12.5 / 16.6, 49 / 36, 324 / 200.  int8: 16 rows 14 / 21,
+  // 28 / 50, 86 / 223; 64 rows 15 / 23, 51 / 52, 283 / 226.  hd 64: 16 rows 11 / 15, 18 / 26, 57 / 85; 24 rows 11 / 15, 22 /
+  // 27, 94 / 86.  So 16 is the last count at which the few-row kernel is ahead everywhere; up to 32 it is within
+  // 10%, and ahead over int8 and short caches.
   if (static_cast<int64_t>(a.max_q) * p.G <= 16 || p.G > 128) {
     p.bm = static_cast<int64_t>(a.max_q) * p.G <= 8 ? 8 : 16;
     p.tile_tokens = p.bm % p.G ? 0 : p.bm / p.G;

@@ -19,8 +19,8 @@
 //               running maximum grew by more than 2^8;
 //   warps 12-15 (int8 cache) turn the codes into bf16 tiles, exactly, one key a thread; k's scale
 //               multiplies the scores and v's the weights, in fp32.
-// Measured: 4 x 509 tokens over up to 4091, 20 heads, 102 us (597 TFLOP/s); 1024 over 8192, 16 heads,
-// 98 us (659; int8 136 us); 1531 over 20011, 32 query and 8 key heads, int8, 793 us (609).  Per 64-key step of
+// Measured: 4 x 509 tokens over up to 4091, 20 heads, 104 us (586 TFLOP/s); 1024 over 8192, 16 heads,
+// 100 us (642; int8 137 us); 1531 over 20011, 32 query and 8 key heads, int8, 809 us (597).  Per 64-key step of
 // 2450 clocks the softmax waits 700 for its scores, takes 260 for the maximum and 1010 for the
 // exponentials; start-up, partial results and the join of split items are a sixth of the 102 us.
 // Other forms, same cases: one stream of two threads a row 115; one S buffer of 128 keys a

@@ -15,8 +15,8 @@
 // tokens at a time and every CTA reads the row's whole history (4 bytes a token, from L2
 // after the first CTA) into them with integer atomics, whose order does not change the
 // counts.  The CTAs' best tokens meet in the first CTA's shared memory.
-// 192 rows of 128003 with 2000 history tokens and 40 biases each: 82 us, 2.4 TB/s of the 8 bytes a
-// logit (55 us with neither, 46 without counts): parts of 8192 tokens alternate counting,
+// 192 rows of 128003 with 2000 history tokens and 40 biases each: 83 us, 2.4 TB/s of the 8 bytes a
+// logit (76 us without the biases, 61 without the history, 48 with neither): parts of 8192 tokens alternate counting,
 // streaming and biases between barriers, and half of all issue slots go to the penalties of
 // vectors that hold a listed token.  Biases and the first history tokens are fetched ahead (89 us
 // without; 8 tokens a thread instead of 4: 87).  A list of the touched tokens that does the

@@ -173,6 +173,8 @@ def attention_paged(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, k
                     want_lse: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Causal attention of the new tokens q [T, heads * hd] over the cache: sequence s owns rows
     q_start[s] .. q_start[s + 1] and the first kv_lens[s] tokens of pages page_table[s], its new tokens last.
+    page_table may be a part of a wider tensor, or one row expanded over the sequences.  Weights keep 15 bits (int8
+    cache: 11) for their product with v where max_q * heads / kv_heads <= 16, 8 where it is more.
     Returns (out [T, heads * hd] bf16, lse2 [T, heads] fp32 or None)."""
     return _ext.attention_paged(q, cache.addr, cache.index, cache.err_ptr, page_table, kv_lens, q_start, heads, workspace.ptr,
                                 workspace.size, workspace.index, max_q, max_kv, window,
