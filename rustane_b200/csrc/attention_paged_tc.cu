@@ -106,11 +106,12 @@ __device__ __forceinline__ void softmax_bar() { asm volatile("bar.sync 1, 256;" 
 // the two softmax warps (one a stream) of TMEM lane quadrant qw
 __device__ __forceinline__ void quad_bar(int qw) { asm volatile("bar.sync %0, 64;" ::"r"(2 + qw) : "memory"); }
 
-// row_attend() 8 keys (of one page) at a time, whose loads and sums over the lanes run side by side: a warp
-// does up to 32 rows over, one after another, while the CTA's other roles wait for it within their limit of
-// 4 s.  4 x 509 rows over 4091 keys, 20 heads, one request's all done over: 20 ms (76 ms with row_attend(); 0.14 ms
-// without a NaN), 0.15 us a key and row: the limit is at 800k keys of one CTA's part.  (The next 8 keys' loads in
-// flight as well: no faster, and its registers cost the ordinary rows 5%.)
+// row_attend() 8 keys (of one page) at a time, whose loads run side by side; the lanes' sums are halved in
+// number at each step, so that 4 lanes end with one key's score.  A warp does up to 32 rows over, one after
+// another, while the CTA's other roles wait for it within their limit of 4 s.  4 x 509 rows over 4091 keys, 20 heads,
+// one request's all done over: 14.4 ms (76 ms with row_attend(), 20 with 8 whole sums; 0.14 ms without a NaN), 0.11
+// us a key and row: the limit is at 1.1M keys of one CTA's part.  (The next 8 keys' loads in flight as well: no
+// faster, and its registers cost the ordinary rows 5%.)
 template <int HD>
 __device__ __noinline__ void redo_row(const Params& p, const int32_t* table, int h, const __nv_bfloat16* qrow, int lo,
                                       int hi, float& m_out, float& l_out, float (&o_out)[HD / 32]) {
@@ -135,44 +136,51 @@ __device__ __noinline__ void redo_row(const Params& p, const int32_t* table, int
   for (int j0 = j_first; j0 < hi; j0 += KB) {
     const int64_t page = checked_page(p, page_next);
     const int64_t at = ((page * p.a.cache.kv_heads + h) << p.page_shift) + (j0 & ((1 << p.page_shift) - 1));
+    // all 8 keys are rows of the page, so they can be loaded whether the row sees them or not
     Row k[KB], v[KB];
 #pragma unroll
-    for (int i = 0; i < KB; ++i) {
-      k[i].x = v[i].x = Pair{};
-      if (j0 + i >= lo && j0 + i < hi) {
-        k[i].x = *reinterpret_cast<const Pair*>(kc + (at + i) * HD + lane * E);
-        v[i].x = *reinterpret_cast<const Pair*>(vc + (at + i) * HD + lane * E);
-      }
-    }
+    for (int i = 0; i < KB; ++i) k[i].x = *reinterpret_cast<const Pair*>(kc + (at + i) * HD + lane * E);
+#pragma unroll
+    for (int i = 0; i < KB; ++i) v[i].x = *reinterpret_cast<const Pair*>(vc + (at + i) * HD + lane * E);
     page_next = entry(j0 + KB);
-    float s[KB], m2 = m;
+    float s[KB];
 #pragma unroll
     for (int i = 0; i < KB; ++i) {
       s[i] = 0.f;
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) s[i] += q[2 * e] * bf16lo(k[i].w[e]) + q[2 * e + 1] * bf16hi(k[i].w[e]);
     }
+    // sums over the lanes, half as many a step: lanes 4 i .. 4 i + 3 end with key i's (bits 4, 3, 2 of the lane)
 #pragma unroll
-    for (int x = 16; x; x >>= 1)
+    for (int n = KB / 2, x = 16; n; n /= 2, x /= 2) {
+      const bool up = lane & x;
 #pragma unroll
-      for (int i = 0; i < KB; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], x);
-#pragma unroll
-    for (int i = 0; i < KB; ++i) {
-      s[i] = j0 + i >= lo && j0 + i < hi ? s[i] * p.scale_log2 : -CUDART_INF_F;
-      m2 = fmaxf(m2, s[i]);
+      for (int i = 0; i < n; ++i) {
+        const float keep = up ? s[i + n] : s[i], give = up ? s[i] : s[i + n];
+        s[i] = keep + __shfl_xor_sync(0xffffffffu, give, x);
+      }
     }
-    const float f = m == m2 ? 1.f : exp2f(m - m2);
+#pragma unroll
+    for (int x = 2; x; x /= 2) s[0] += __shfl_xor_sync(0xffffffffu, s[0], x);
+    const int mine = j0 + (lane >> 2);
+    const float score = mine >= lo && mine < hi ? s[0] * p.scale_log2 : -CUDART_INF_F;
+    float m2 = score;
+#pragma unroll
+    for (int x = 4; x < 32; x *= 2) m2 = fmaxf(m2, __shfl_xor_sync(0xffffffffu, m2, x));
+    m2 = fmaxf(m, m2);
+    const float f = m == m2 ? 1.f : exp2f(m - m2), weight = score == -CUDART_INF_F ? 0.f : exp2f(score - m2);
     l *= f;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] *= f;
 #pragma unroll
     for (int i = 0; i < KB; ++i) {
-      const float pj = s[i] == -CUDART_INF_F ? 0.f : exp2f(s[i] - m2);
+      const float pj = __shfl_sync(0xffffffffu, weight, 4 * i);
+      const bool in = j0 + i >= lo && j0 + i < hi;  // an unseen v may be NaN
       l += pj;
 #pragma unroll
       for (int e = 0; e < E / 2; ++e) {
-        o[2 * e] += pj * bf16lo(v[i].w[e]);
-        o[2 * e + 1] += pj * bf16hi(v[i].w[e]);
+        o[2 * e] += pj * (in ? bf16lo(v[i].w[e]) : 0.f);
+        o[2 * e + 1] += pj * (in ? bf16hi(v[i].w[e]) : 0.f);
       }
     }
     m = m2;
